@@ -141,6 +141,54 @@ starneig_error_t starneig_amd_dgemm_device(
     double const *dA, int ldA, double const *dB, int ldB, double beta,
     double *dC, int ldC, void *stream);
 
+/* ---- products over ragged groups of columns, and in 8-bit integers ---------------------------------------
+ * The products of layers that have a matrix per group of columns (experts and the tokens sent to them, windows and
+ * the columns right of them).  Column-major like everything here: a token is a column, so a row-major array
+ * (tokens, features) is passed as it lies, and row-major weights (out, in) are A with transA = 'T'.
+ * Group g owns the columns [dOffsets[g], dOffsets[g + 1]) of the n columns; dOffsets holds groups + 1 ints in DEVICE
+ * memory and may be written on `stream` just before (prefix sums of a router's counts): the host does not read it.
+ * Groups may be empty; columns in front of the first and behind the last group belong to none.  An offset outside
+ * [0, n] counts as the nearer end, one below its predecessor as its predecessor.
+ * The calls enqueue on `stream` and return; they hold no state, no workspace and no lock, so they may run
+ * on several streams at once and be captured into graphs.  All pointers are on the current device and aligned to their
+ * elements; outputs must not overlap inputs.  16-byte aligned columns (pointer and leading dimension) are read fastest.
+ * fp16 / bf16 sums are held in fp32 and rounded once, fp64 sums as in starneig_amd_dgemm_device; equal calls give
+ * equal bits.  A return value of -i marks the i-th argument, STARNEIG_GENERIC_ERROR a launch that failed (sizes beyond
+ * 2^32 threads included). */
+enum starneig_amd_type { STARNEIG_AMD_F64 = 0, STARNEIG_AMD_F32 = 1, STARNEIG_AMD_BF16 = 2, STARNEIG_AMD_F16 = 3 };
+
+/* C(:, c) = op(A_g) B(:, c) for every column c of group g.  op(A_g): m x k at dA + g strideA elements (strideA 0: one
+ * matrix for all); transA 'N' = stored m x k, 'T' = stored k x m.  B: k x n, C: m x n; columns of C that belong to no
+ * group stay as they are.  type (of A, B and C): F64, BF16 or F16.
+ * With A's weights, 'T' is a layer's forward product and 'N' the gradient of its inputs. */
+starneig_error_t starneig_amd_grouped_gemm_device(
+    int type, char transA, int groups, int m, int n, int k, int const *dOffsets,
+    void const *dA, int ldA, long strideA, void const *dB, int ldB, void *dC, int ldC, void *stream);
+
+/* D_g = X_g Y_g^T + beta D_g, the sum over the columns of group g: the gradient of A_g with X = B and Y = the gradient
+ * of C (transA = 'T'), or X and Y swapped ('N').  X: m x k, Y: n x k (k: all columns), D_g: m x n at dD + g strideD
+ * elements.  An empty group gives beta D_g; beta = 0 does not read D.  typeD: `type`, or F32 for BF16 / F16. */
+starneig_error_t starneig_amd_grouped_outer_device(
+    int type, int typeD, int groups, int m, int n, int k, int const *dOffsets,
+    void const *dX, int ldX, void const *dY, int ldY, double beta, void *dD, int ldD, long strideD, void *stream);
+
+/* Q(:, c) = rint(X(:, c) / s_c), s_c = dScale[c] = max_i |X(i, c)| / 127 in IEEE fp32, halves to even.  X: k x n of type F32, BF16 or F16.
+ * A column of zeros gets s = 0 and Q = 0; one that holds an infinity or a NaN gets that s and Q = 0 (its product is NaN). */
+starneig_error_t starneig_amd_quantize_i8_device(
+    int type, int k, int n, void const *dX, int ldX, signed char *dQ, int ldQ, float *dScale, void *stream);
+
+/* C(r, c) = (sum_i A(i, r) B(i, c)) dScaleA[r] dScaleB[c]: A k x m (a channel a column: row-major weights (out, in)), B k x n,
+ * both 8-bit integers; C m x n of typeC F32, BF16 or F16.  The sum is exact (k <= 131071); the scales multiply it in fp32 in this order. */
+starneig_error_t starneig_amd_gemm_i8_device(
+    int typeC, int m, int n, int k, signed char const *dA, int ldA, float const *dScaleA,
+    signed char const *dB, int ldB, float const *dScaleB, void *dC, int ldC, void *stream);
+
+/* The same with a matrix and its scales per group: A_g at dA + g strideA, its scales at dScaleA + g strideScaleA. */
+starneig_error_t starneig_amd_grouped_gemm_i8_device(
+    int typeC, int groups, int m, int n, int k, int const *dOffsets,
+    signed char const *dA, int ldA, long strideA, float const *dScaleA, long strideScaleA,
+    signed char const *dB, int ldB, float const *dScaleB, void *dC, int ldC, void *stream);
+
 /* The reference test driver's LCG inputs generated directly in HBM
  * (test/common/common.c:56-59, test/common/init.c:93-120):
  * mode 0 = prand/PRAND_MAX in [0,1] ("fullpos"), mode 1 = 2*prand/PRAND_MAX-1. */

@@ -6,6 +6,7 @@
 #include "tuning.h"
 #include <chrono>
 #include "schur_host.h"
+#include "products.h"
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -942,6 +943,136 @@ SN_API starneig_error_t starneig_amd_dgemm_device(
     if (!g_node.initialized) return STARNEIG_NOT_INITIALIZED;
     sn::dgemm((hipStream_t)stream, transA, transB, m, n, k, alpha, dA, ldA, dB, ldB, beta, dC, ldC);
     return STARNEIG_SUCCESS;
+}
+
+// ---- grouped and 8-bit products ---------------------------------------------------------------------------------
+
+namespace {
+int product_size(int type) { return type == STARNEIG_AMD_F64 ? 8 : type == STARNEIG_AMD_F32 ? 4 : type == STARNEIG_AMD_BF16 || type == STARNEIG_AMD_F16 ? 2 : 0; }
+bool bad_pointer(void const *p, int align) { return p == NULL || (uintptr_t)p % align != 0; }
+starneig_error_t launched(hipError_t e) { return e == hipSuccess ? STARNEIG_SUCCESS : STARNEIG_GENERIC_ERROR; }
+}
+
+SN_API starneig_error_t starneig_amd_grouped_gemm_device(
+    int type, char transA, int groups, int m, int n, int k, int const *dOffsets,
+    void const *dA, int ldA, long strideA, void const *dB, int ldB, void *dC, int ldC, void *stream)
+{
+    bool const ta = transA == 'T' || transA == 't';
+    int const size = product_size(type);
+    if (size == 0 || type == STARNEIG_AMD_F32) return -1;
+    if (!ta && transA != 'N' && transA != 'n') return -2;
+    if (groups < 1) return -3;
+    if (m < 0) return -4;
+    if (n < 0) return -5;
+    if (k < 0) return -6;
+    bool const some = m > 0 && n > 0;
+    if (some && bad_pointer(dOffsets, 4)) return -7;
+    if (some && k > 0 && bad_pointer(dA, size)) return -8;
+    if (ldA < std::max(1, ta ? k : m)) return -9;
+    if (strideA < 0) return -10;
+    if (some && k > 0 && bad_pointer(dB, size)) return -11;
+    if (ldB < std::max(1, k)) return -12;
+    if (some && bad_pointer(dC, size)) return -13;
+    if (ldC < std::max(1, m)) return -14;
+    if (!g_node.initialized) return STARNEIG_NOT_INITIALIZED;
+    if (!some) return STARNEIG_SUCCESS;
+    return launched(sn::grouped_gemm((hipStream_t)stream, (sn::ProductType)type, ta, groups, m, n, k, dOffsets, dA, ldA, strideA, dB, ldB, dC, ldC));
+}
+
+SN_API starneig_error_t starneig_amd_grouped_outer_device(
+    int type, int typeD, int groups, int m, int n, int k, int const *dOffsets,
+    void const *dX, int ldX, void const *dY, int ldY, double beta, void *dD, int ldD, long strideD, void *stream)
+{
+    int const size = product_size(type);
+    if (size == 0 || type == STARNEIG_AMD_F32) return -1;
+    if (typeD != type && (typeD != STARNEIG_AMD_F32 || type == STARNEIG_AMD_F64)) return -2;
+    if (groups < 1) return -3;
+    if (m < 0) return -4;
+    if (n < 0) return -5;
+    if (k < 0) return -6;
+    bool const some = m > 0 && n > 0;
+    if (some && bad_pointer(dOffsets, 4)) return -7;
+    if (some && k > 0 && bad_pointer(dX, size)) return -8;
+    if (ldX < std::max(1, m)) return -9;
+    if (some && k > 0 && bad_pointer(dY, size)) return -10;
+    if (ldY < std::max(1, n)) return -11;
+    if (some && bad_pointer(dD, product_size(typeD))) return -13;
+    if (ldD < std::max(1, m)) return -14;
+    // (the groups' matrices must not overlap)
+    if (some && groups > 1 && strideD < (long)(n - 1) * ldD + m) return -15;
+    if (!g_node.initialized) return STARNEIG_NOT_INITIALIZED;
+    if (!some) return STARNEIG_SUCCESS;
+    return launched(sn::grouped_outer((hipStream_t)stream, (sn::ProductType)type, (sn::ProductType)typeD, groups, m, n, k, dOffsets,
+        dX, ldX, dY, ldY, beta, dD, ldD, strideD));
+}
+
+SN_API starneig_error_t starneig_amd_quantize_i8_device(
+    int type, int k, int n, void const *dX, int ldX, signed char *dQ, int ldQ, float *dScale, void *stream)
+{
+    int const size = product_size(type);
+    if (size == 0 || type == STARNEIG_AMD_F64) return -1;
+    if (k < 0) return -2;
+    if (n < 0) return -3;
+    if (n > 0 && k > 0 && bad_pointer(dX, size)) return -4;
+    if (ldX < std::max(1, k)) return -5;
+    if (n > 0 && k > 0 && bad_pointer(dQ, 1)) return -6;
+    if (ldQ < std::max(1, k)) return -7;
+    if (n > 0 && bad_pointer(dScale, 4)) return -8;
+    if (!g_node.initialized) return STARNEIG_NOT_INITIALIZED;
+    if (n == 0) return STARNEIG_SUCCESS;
+    return launched(sn::quantize_i8((hipStream_t)stream, (sn::ProductType)type, k, n, dX, ldX, dQ, ldQ, dScale));
+}
+
+SN_API starneig_error_t starneig_amd_gemm_i8_device(
+    int typeC, int m, int n, int k, signed char const *dA, int ldA, float const *dScaleA,
+    signed char const *dB, int ldB, float const *dScaleB, void *dC, int ldC, void *stream)
+{
+    int const size = product_size(typeC);
+    if (size == 0 || typeC == STARNEIG_AMD_F64) return -1;
+    if (m < 0) return -2;
+    if (n < 0) return -3;
+    if (k < 0 || k > 131071) return -4;         // 131071 * 128 * 128 < 2^31
+    bool const some = m > 0 && n > 0;
+    if (some && k > 0 && bad_pointer(dA, 1)) return -5;
+    if (ldA < std::max(1, k)) return -6;
+    if (some && bad_pointer(dScaleA, 4)) return -7;
+    if (some && k > 0 && bad_pointer(dB, 1)) return -8;
+    if (ldB < std::max(1, k)) return -9;
+    if (some && bad_pointer(dScaleB, 4)) return -10;
+    if (some && bad_pointer(dC, size)) return -11;
+    if (ldC < std::max(1, m)) return -12;
+    if (!g_node.initialized) return STARNEIG_NOT_INITIALIZED;
+    if (!some) return STARNEIG_SUCCESS;
+    return launched(sn::gemm_i8((hipStream_t)stream, (sn::ProductType)typeC, 1, m, n, k, NULL, dA, ldA, 0, dScaleA, 0, dB, ldB, dScaleB, dC, ldC));
+}
+
+SN_API starneig_error_t starneig_amd_grouped_gemm_i8_device(
+    int typeC, int groups, int m, int n, int k, int const *dOffsets,
+    signed char const *dA, int ldA, long strideA, float const *dScaleA, long strideScaleA,
+    signed char const *dB, int ldB, float const *dScaleB, void *dC, int ldC, void *stream)
+{
+    int const size = product_size(typeC);
+    if (size == 0 || typeC == STARNEIG_AMD_F64) return -1;
+    if (groups < 1) return -2;
+    if (m < 0) return -3;
+    if (n < 0) return -4;
+    if (k < 0 || k > 131071) return -5;
+    bool const some = m > 0 && n > 0;
+    if (some && bad_pointer(dOffsets, 4)) return -6;
+    if (some && k > 0 && bad_pointer(dA, 1)) return -7;
+    if (ldA < std::max(1, k)) return -8;
+    if (strideA < 0) return -9;
+    if (some && bad_pointer(dScaleA, 4)) return -10;
+    if (strideScaleA < 0) return -11;
+    if (some && k > 0 && bad_pointer(dB, 1)) return -12;
+    if (ldB < std::max(1, k)) return -13;
+    if (some && bad_pointer(dScaleB, 4)) return -14;
+    if (some && bad_pointer(dC, size)) return -15;
+    if (ldC < std::max(1, m)) return -16;
+    if (!g_node.initialized) return STARNEIG_NOT_INITIALIZED;
+    if (!some) return STARNEIG_SUCCESS;
+    return launched(sn::gemm_i8((hipStream_t)stream, (sn::ProductType)typeC, groups, m, n, k, dOffsets, dA, ldA, strideA, dScaleA, strideScaleA,
+        dB, ldB, dScaleB, dC, ldC));
 }
 
 SN_API starneig_error_t starneig_amd_lcg_fill_device(
