@@ -1,25 +1,46 @@
 // The tile of the grouped and the 8-bit products: BM x BN outputs of one workgroup from the matrix cores, operands through LDS.
 //
-// A k-tile is 128 bytes of the inner index (64 numbers of 16 bits, 128 of 8).  An operand lies in memory with the inner index
-// contiguous ("K": weights of a forward product, tokens) or with the outer index contiguous (weights of an input
+// A k-tile is 128 bytes of the inner index (64 numbers of 16 bits, 128 of 8): a cache line.  An operand lies in memory with the inner index
+// contiguous ("K": weights of a forward product, tokens) or with the outer index contiguous ("MN": weights of an input
 // gradient, both operands of a weight gradient); LDS holds a straight copy of what is contiguous, in 16-byte chunks:
 //   K:  [outer][8 chunks of inner],          chunk c of row r at place c ^ swizzle_k(r); fragments by ds_read_b128
 //   MN: [64 inner rows][outer / 8 chunks],   chunk c of row k at place c ^ swizzle_mn(k); fragments by ds_read_b64_tr_b16, which
 //       hands lane i of 16 the four numbers of its column out of four rows
 // Both leave the fragment reads without bank conflicts.
 //
-// Outer index of lane i of a fragment: the four fragments t of 64 rows interleave, row = 16 (i >> 2) + 4 t + (i & 3).  The accumulators of the four
-// fragments then hold 16 consecutive rows of a column per lane, and a column's 64 rows are stored as whole lines.
+// The two fragments t of 64 rows interleave.  K: lane i holds row 8 (i >> 2) + 4 t + (i & 3), so that the accumulators of the two hold eight
+// consecutive rows of a column per lane.  MN: row 32 t + i, whose reads touch every bank; four consecutive rows per lane.
 #pragma once
 #include "product_types.h"
 
 namespace sn {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 // How an operand is brought into LDS: DIRECT = buffer loads that write LDS themselves (16-byte aligned columns, whole chunks), no registers and
 // no LDS instructions; STAGED = through registers, any alignment and any extent.
 enum Feed { DIRECT, STAGED };
+
+// A buffer of `bytes` bytes from `p` on: loads from offsets beyond it give zeros.
+__device__ __forceinline__ i32x4 buffer(void const *p, int bytes)
+{
+    unsigned long long const at = (unsigned long long)p;
+    return (i32x4){__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff), bytes, 0x00020000};
+}
+// 16 bytes a lane from `offset` of the buffer into LDS: the wave's from `to` (the same in all lanes) on, in the lanes' order.  In assembly: with the
+// builtin the compiler waits for all loads before the next transposing LDS read, which it takes to read what they write; here the
+// barriers order them.  The compiler does not look inside, so the five wait states are here that a load needs behind a vector
+// instruction (v_readfirstlane) that has written one of its scalar registers, and the one behind m0.
+__device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, int to)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(to), "v"(offset), "s"(buffer) : "memory");
+}
+// threadIdx.x for what is computed once a tile: the compiler must not compute it before the loops and hold it in registers meanwhile
+__device__ __forceinline__ int thread_now() { int t = threadIdx.x; asm volatile("" : "+v"(t)); return t; }
+__device__ __forceinline__ int wave_number() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 template <typename T, int ROWS, bool K, int THREADS>
 struct Operand {
@@ -29,8 +50,12 @@ struct Operand {
     static constexpr int LOADS = ROWS * 8 / THREADS;        // chunks a thread brings
     static constexpr int CR = ROWS / EL;                    // MN: chunks a row
 
-    static __device__ __forceinline__ int swizzle_k(int r) { return (r & 3) | (r >> 2 & 4); }
-    static __device__ __forceinline__ int swizzle_mn(int k) { return (k & 1) | (k & 2) << 2; }
+    // (ds_read_b128 serves 16 lanes at a time: 0-3, 12-15, 20-27; 4-11, 16-19, 28-31; and so on; ds_read_b64_tr_b16 32)
+    static __device__ __forceinline__ int swizzle_k(int r) { return (r >> 1 & 1) | (r >> 3 & 6); }
+    static __device__ __forceinline__ int swizzle_mn(int k) { return (k & 3) << 2; }
+
+    // row of lane i of fragment t of 64 rows
+    static __device__ __forceinline__ int row(int i, int t) { return K ? 8 * (i >> 2) + 4 * t + (i & 3) : 32 * t + i; }
 
     // outer and inner position, inside the tile, of the chunk that goes to place e
     static __device__ __forceinline__ void chunk(int e, int &outer, int &inner)
@@ -39,29 +64,29 @@ struct Operand {
         else   { inner = e / CR; outer = ((e % CR) ^ swizzle_mn(inner)) * EL; }
     }
 
-    // fragment t of the 64 rows from `row0`, 64 bytes of inner index number `half`
-    static __device__ __forceinline__ i32x4 fragment(char const *lds, int row0, int t, int half)
+    // fragment t of the 64 rows from `row0`, 32 bytes of inner index number `step` of 4
+    static __device__ __forceinline__ i32x4 fragment(lds_char const *lds, int row0, int t, int step)
     {
-        int const lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+        int const lane = threadIdx.x & 63, q = lane >> 5;
         if constexpr (K) {
-            int const r = row0 + 16 * (i >> 2) + 4 * t + (i & 3), c = half * 4 + q;
-            return *(i32x4 const *)(lds + r * 128 + ((c ^ swizzle_k(r)) << 4));
+            int const r = row(lane & 31, t);
+            return *(lds_i32x4 const *)(lds + (row0 + r) * 128 + (((2 * step + q) ^ swizzle_k(r)) << 4));
         } else {
-            // lane 4 j + c of the 16 names four numbers of row j: rows 16 c + 4 t ...; it gets column i = 4 c' + e of all four
-            int const j = i >> 2, c = i & 3;
+            // lane 4 j + c of 16 names four numbers of row j of four; it gets its own column's of all four rows
+            int const j = lane >> 2 & 3, c = lane & 3, outer = row0 + row((lane & 16) + 4 * c, t);
             u32x2 part[2];
             #pragma unroll
             for (int h = 0; h < 2; h++) {
-                int const k = half * 32 + 8 * q + 4 * h + j, outer = row0 + 16 * c + 4 * t;
-                char const *const at = lds + k * (ROWS * 2) + (((outer >> 3) ^ swizzle_mn(k)) << 4) + (outer & 4) * 2;
-                part[h] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at)));
+                int const k = 16 * step + 8 * q + 4 * h + j;
+                lds_char const *const at = lds + k * (ROWS * 2) + (((outer >> 3) ^ swizzle_mn(k)) << 4) + (outer & 4) * 2;
+                part[h] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at));
             }
             return (i32x4){(int)part[0].x, (int)part[0].y, (int)part[1].x, (int)part[1].y};
         }
     }
 };
 
-// One operand of one tile on its way into LDS.  `base`: its element (outer 0, inner 0) of the tile; `outers`: how many outer positions
+// One operand on its way into LDS, tile after tile.  set(): `base`: its element (outer 0, inner 0) of the tile; `outers`: how many outer positions
 // exist from there (may exceed ROWS); `k`: inner terms in all; `ld`: distance of the positions that are not contiguous.
 template <typename T, int ROWS, bool K, int THREADS, Feed FEED> struct Stream;
 
@@ -72,191 +97,318 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
     long step;                      // MN: numbers between k-tiles
     int k;
     unsigned at[O::LOADS];          // byte offsets of the thread's chunks; beyond the buffer where there is nothing to read
-    int inner[K ? 1 : O::LOADS];
 
-    __device__ __forceinline__ Stream(T const *base_, int outers, int k_, long ld) : base(base_), step(ld * O::KT), k(k_)
+    __device__ __forceinline__ void set(T const *base_, int outers, int k_, long ld, int)
     {
+        base = base_; step = ld * O::KT; k = k_;
+        int const thread = thread_now();
         #pragma unroll
         for (int s = 0; s < O::LOADS; s++) {
             int outer, in;
-            O::chunk(s * THREADS + threadIdx.x, outer, in);
-            if (K) { at[s] = outer < outers ? (unsigned)(outer * (int)(ld * sizeof(T)) + in * (int)sizeof(T)) : 0x80000000u; inner[0] = in; }
-            else   { at[s] = outer < outers ? (unsigned)(in * (int)(ld * sizeof(T)) + outer * (int)sizeof(T)) : 0x80000000u; inner[K ? 0 : s] = in; }
+            O::chunk(s * THREADS + thread, outer, in);
+            int const far = K ? outer : in, near = K ? in : outer;
+            at[s] = outer < outers ? (unsigned)(far * (int)(ld * sizeof(T)) + near * (int)sizeof(T)) : 0x80000000u;
         }
     }
-    // starts bringing k-tile kt to `lds`.  Offsets from 2^31 on read zeros (the buffer's length is 2^31 - 1): positions past the outer
-    // end, and inner chunks past k.
-    __device__ __forceinline__ void fetch(char *lds, int kt) const
+    // Loads 0 ... LOADS - 1 of k-tile kt to `lds`, after begin(kt); k-tiles are fetched in order.  Offsets from 2^31 on read zeros: positions
+    // past the outer end, and, from the k-tile on that k cuts, the chunks past k.  Behind the last k-tile the buffer is empty.
+    i32x4 from;
+    __device__ __forceinline__ void begin(int kt)
     {
-        T const *const from = K ? base + (long)kt * O::KT : base + kt * step;
-        __amdgpu_buffer_rsrc_t const r = __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, 0x7fffffff, 0x00020000);
         int const left = k - kt * O::KT;
-        #pragma unroll
-        for (int s = 0; s < O::LOADS; s++) {
-            unsigned v = at[s];
-            if (left < O::KT) v = inner[K ? 0 : s] < left ? v : 0x80000000u;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (s * THREADS + (int)(threadIdx.x & ~63u)) * 16),
-                16, (int)v, 0, 0, 0);
+        if (left < O::KT && left > 0) {
+            int const thread = thread_now();
+            #pragma unroll
+            for (int s = 0; s < O::LOADS; s++) {
+                int outer, inner;
+                O::chunk(s * THREADS + thread, outer, inner);
+                if (inner >= left) at[s] = 0x80000000u;
+            }
         }
+        from = buffer(K ? base + (long)kt * O::KT : base + kt * step, left > 0 ? 0x7fffffff : 0);
     }
-    __device__ __forceinline__ void put(char *) const {}
+    __device__ __forceinline__ void load(int lds, int s) const { load_to_lds(from, at[s], lds + wave_number() * 1024 + s * THREADS * 16); }
+    __device__ __forceinline__ void fetch(int lds, int kt)
+    {
+        begin(kt);
+        #pragma unroll
+        for (int s = 0; s < O::LOADS; s++) load(lds, s);
+    }
+    __device__ __forceinline__ void put(lds_char *, int) const {}
 };
 
+// v moved down by `bits`, zeros from above
+__device__ __forceinline__ i32x4 moved_down(i32x4 v, int bits)
+{
+    typedef unsigned long long u64x2 __attribute__((ext_vector_type(2)));
+    u64x2 w = __builtin_bit_cast(u64x2, v);
+    if (bits >= 64) { w.x = w.y; w.y = 0; bits -= 64; }
+    if (bits >= 64) w.x = 0;
+    else if (bits > 0) { w.x = w.x >> bits | w.y << (64 - bits); w.y >>= bits; }
+    return __builtin_bit_cast(i32x4, w);
+}
+
+// Every load is of a whole chunk inside the operand: positions that are not there read others in their place, and a chunk that the end
+// cuts is read from where it ends there.  put() moves such a chunk to its place and zeroes what has to be zero: the
+// inner terms past k.  (Outer positions past the end only meet outputs that are not stored.)  An operand of less than a
+// chunk of contiguous numbers is read number by number.
 template <typename T, int ROWS, bool K, int THREADS>
 struct Stream<T, ROWS, K, THREADS, STAGED> {
     using O = Operand<T, ROWS, K, THREADS>;
     T const *base;
     long ld;
     int outers, k;
+    bool tiny;
     i32x4 held[O::LOADS];
 
-    __device__ __forceinline__ Stream(T const *base_, int outers_, int k_, long ld_) : base(base_), ld(ld_), outers(outers_), k(k_) {}
-
-    __device__ __forceinline__ void fetch(char *, int kt)
+    // `before`: contiguous positions in front of `base` (MN: the tile's first row)
+    __device__ __forceinline__ void set(T const *base_, int outers_, int k_, long ld_, int before)
     {
-        int const left = k - kt * O::KT;
-        T const *const from = K ? base + (long)kt * O::KT : base + (long)kt * O::KT * ld;
+        base = base_; ld = ld_; outers = outers_; k = k_;
+        tiny = K ? k_ < O::EL : outers_ + before < O::EL;
+    }
+
+    __device__ __forceinline__ void fetch(int, int kt)
+    {
+        if (kt * O::KT >= k) return;
         #pragma unroll
         for (int s = 0; s < O::LOADS; s++) {
             int outer, inner;
             O::chunk(s * THREADS + threadIdx.x, outer, inner);
-            // (whole chunks by one load from wherever they start; a chunk that the end cuts, number by number)
-            bool const whole = K ? inner + O::EL <= left && outer < outers : outer + O::EL <= outers && inner < left;
-            T const *const p = K ? from + outer * ld + inner : from + inner * ld + outer;
-            i32x4 v = {0, 0, 0, 0};
-            if (whole) __builtin_memcpy(&v, p, 16);
-            else {
-                int const rest = K ? (outer < outers ? left - inner : 0) : (inner < left ? outers - outer : 0);
-                T one[O::EL];
-                #pragma unroll
-                for (int e = 0; e < O::EL; e++) one[e] = e < rest ? p[e] : (T)0;
-                __builtin_memcpy(&v, one, 16);
+            inner += kt * O::KT;
+            if (!tiny) {
+                T const *const p = K ? base + min(outer, outers - 1) * ld + min(inner, k - O::EL)
+                                     : base + min(inner, k - 1) * ld + min(outer, outers - O::EL);
+                __builtin_memcpy(&held[s], p, 16);
+            } else {
+                T const *const p = K ? base + min(outer, outers - 1) * ld : base + min(inner, k - 1) * ld;
+                int const from = K ? inner : outer, end = K ? k : outers;
+                unsigned long long w[2] = {0, 0};
+                #pragma unroll 1
+                for (int e = 0; e < O::EL; e++) {
+                    T const one = p[min(from + e, end - 1)];
+                    unsigned long long bits = 0;
+                    __builtin_memcpy(&bits, &one, sizeof one);
+                    int const at = e * 8 * (int)sizeof(T);
+                    if (from + e < end) w[at >> 6] |= bits << (at & 63);
+                }
+                __builtin_memcpy(&held[s], w, 16);
             }
-            held[s] = v;
         }
     }
-    __device__ __forceinline__ void put(char *lds) const
+    __device__ __forceinline__ void put(lds_char *lds, int kt) const
     {
+        if (kt * O::KT >= k) return;
+        bool const cut = !tiny && (K ? (kt + 1) * O::KT > k : outers < ROWS || (kt + 1) * O::KT > k);
         #pragma unroll
-        for (int s = 0; s < O::LOADS; s++) *(i32x4 *)(lds + (s * THREADS + threadIdx.x) * 16) = held[s];
+        for (int s = 0; s < O::LOADS; s++) {
+            i32x4 v = held[s];
+            if (cut || (tiny && !K)) {
+                int outer, inner;
+                O::chunk(s * THREADS + threadIdx.x, outer, inner);
+                inner += kt * O::KT;
+                int const over = tiny ? 0 : K ? inner - (k - O::EL) : outer - (outers - O::EL);
+                if (over > 0) v = moved_down(v, min(over, O::EL) * 8 * (int)sizeof(T));
+                if (!K && inner >= k) v = (i32x4){0, 0, 0, 0};
+            }
+            *(lds_i32x4 *)(lds + (s * THREADS + threadIdx.x) * 16) = v;
+        }
     }
+};
+
+// DIRECT: LDS holds five operands of k-tiles (A, B, A, B, A ... in turn), so that one and a half k-tiles are on their way while one is
+// multiplied.  STAGED: two k-tiles, one in registers on its way.
+// What a tile is the product of.  rows / cols: outputs that exist from its corner on, which is (r0, c0); k: inner terms.
+template <typename T>
+struct Plan {
+    T const *A, *B;
+    long lda, ldb;
+    int rows, cols, k, r0, c0;
 };
 
 template <typename T, int BM_, int BN_, int WAVES_M_, int WAVES_N_, bool AK_, bool BK_, Feed FEED_>
 struct ProductTile {
     static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, THREADS = 64 * WAVES_M * WAVES_N;
     static constexpr int MB = BM / WAVES_M / 64, NB = BN / WAVES_N / 64;     // 64 x 64 blocks a wave
+    static_assert(BM == BN, "the places in LDS are of one size");
     typedef typename Mfma<T>::Acc Acc;
     using OA = Operand<T, BM, AK_, THREADS>;
     using OB = Operand<T, BN, BK_, THREADS>;
-    static constexpr int STAGE = OA::BYTES + OB::BYTES, LDS_BYTES = 2 * STAGE;
+    static constexpr int PLACE = OA::BYTES, PLACES = FEED_ == DIRECT ? 5 : 4, LDS_BYTES = PLACES * PLACE;
     static constexpr int KT = OA::KT;
     static constexpr bool A_K = AK_;
+    static constexpr int PER_SIMD = MB * NB > 2 ? 1 : 2;        // waves
 
-    Acc acc[MB][4][NB][4];
+    Acc acc[MB][2][NB][2];
 
-    __device__ __forceinline__ void multiply(char const *lds)
+    // the operands of half a k-tile in registers
+    struct Fragments { i32x4 a[2][MB][2], b[2][NB][2]; };
+
+    static constexpr int READS = 4 * (MB + NB), PRODUCTS = 8 * MB * NB;         // of half a k-tile
+    static __device__ __forceinline__ void read(Fragments &f, lds_char const *la, lds_char const *lb, int half, int r)
     {
-        int const wave = threadIdx.x >> 6, m0 = wave % WAVES_M * (BM / WAVES_M), n0 = wave / WAVES_M * (BN / WAVES_N);
+        int const wave = wave_number(), m0 = wave % WAVES_M * (BM / WAVES_M), n0 = wave / WAVES_M * (BN / WAVES_N);
+        int const s = r / (2 * (MB + NB)), i = r % (2 * (MB + NB)), x = i / 2 - NB, y = i / 2, t = i % 2;
+        if (y < NB) f.b[s][y][t] = OB::fragment(lb, n0 + 64 * y, t, 2 * half + s);
+        else        f.a[s][x][t] = OA::fragment(la, m0 + 64 * x, t, 2 * half + s);
+    }
+    __device__ __forceinline__ void multiply(Fragments const &f, int p)
+    {
+        int const s = p / (PRODUCTS / 2), i = p % (PRODUCTS / 2), x = i / (4 * NB), t = i / (2 * NB) % 2, y = i / 2 % NB, u = i % 2;
+        acc[x][t][y][u] = Mfma<T>::mul(f.a[s][x][t], f.b[s][y][u], acc[x][t][y][u]);
+    }
+    // The products of f's half k-tile, and between them, evenly, the reads of the next one into g and the loads of a whole one: a wave issues in order,
+    // and loads in a bunch would hold the products behind them up for as long as the address units need for all of them.
+    template <typename S>
+    __device__ __forceinline__ void turn(Fragments const &f, Fragments &g, lds_char const *la, lds_char const *lb, int half, S &stream, int place)
+    {
+        constexpr int LOADS = S::O::LOADS, LAST = PRODUCTS - (PRODUCTS >= 16 ? 6 : 2);       // the reads early: the next turn begins with what they bring
         #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            // (one half's fragments at a time: without it both are loaded first, and the 256 x 256 tile spills)
-            if (half) __builtin_amdgcn_sched_barrier(0);
-            i32x4 a[MB][4], b[NB][4];
+        for (int p = 0; p < PRODUCTS; p++) {
             #pragma unroll
-            for (int y = 0; y < NB; y++)
-                #pragma unroll
-                for (int t = 0; t < 4; t++) b[y][t] = OB::fragment(lds + OA::BYTES, n0 + 64 * y, t, half);
+            for (int r = 0; r < READS; r++) if (r * LAST / READS == p) read(g, la, lb, half, r);
+            multiply(f, p);
             #pragma unroll
-            for (int x = 0; x < MB; x++)
-                #pragma unroll
-                for (int t = 0; t < 4; t++) a[x][t] = OA::fragment(lds, m0 + 64 * x, t, half);
+            for (int l = 0; l < LOADS; l++) if ((2 * l + 1) * PRODUCTS / (2 * LOADS) == p) stream.load(place, l);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // All but the last LOADS loads of every wave have landed, and every wave has read what it has asked LDS for.
+    template <int LOADS>
+    static __device__ __forceinline__ void meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(LOADS) : "memory"); }
+
+    Stream<T, BM, AK_, THREADS, FEED_> a;
+    Stream<T, BN, BK_, THREADS, FEED_> b;
+    Fragments f[FEED_ == DIRECT ? 2 : 1];
+    int now;
+
+    // DIRECT: k-tiles of a tile, at least the two that are fetched ahead (what is past k is zero)
+    static __device__ __forceinline__ int tiles_of(int k) { int const t = (k + KT - 1) / KT; return FEED_ == DIRECT ? max(t, 2) : t; }
+    static __device__ __forceinline__ int after(int place, int n) { place += n * PLACE; return place >= LDS_BYTES ? place - LDS_BYTES : place; }
+    __device__ __forceinline__ void set_a(Plan<T> const &p) { a.set(p.A, p.rows, p.k, p.lda, p.r0); }
+    __device__ __forceinline__ void set_b(Plan<T> const &p) { b.set(p.B, p.cols, p.k, p.ldb, p.c0); }
+
+    // before the first tile
+    __device__ __forceinline__ void start(Plan<T> const &p, char *shared)
+    {
+        lds_char *const lds = (lds_char *)shared;
+        set_a(p); set_b(p);
+        if constexpr (FEED_ == DIRECT) {
+            int const lds0 = __builtin_amdgcn_readfirstlane((int)(unsigned long long)lds);
+            a.fetch(lds0, 0); b.fetch(lds0 + PLACE, 0); a.fetch(lds0 + 2 * PLACE, 1); b.fetch(lds0 + 3 * PLACE, 1);
+            meet<OA::LOADS + OB::LOADS>();
             #pragma unroll
-            for (int x = 0; x < MB; x++)
-                #pragma unroll
-                for (int t = 0; t < 4; t++)
-                    #pragma unroll
-                    for (int y = 0; y < NB; y++)
-                        #pragma unroll
-                        for (int u = 0; u < 4; u++) acc[x][t][y][u] = Mfma<T>::mul(a[x][t], b[y][u], acc[x][t][y][u]);
+            for (int r = 0; r < READS; r++) read(f[0], lds, lds + PLACE, 0, r);
+            now = 0;
         }
     }
 
-    // acc = sum over the k inner terms; rows / cols: outputs that exist from the tile's corner on
-    __device__ __forceinline__ void run(T const *A, long lda, int rows, T const *B, long ldb, int cols, int k, char *lds)
+    // acc = the tile p; where `next` is another, its loads have begun when this one's products end (otherwise it is empty: k = 0)
+    __device__ __forceinline__ void run(Plan<T> const &p, Plan<T> const &next, char *shared)
     {
-        Stream<T, BM, AK_, THREADS, FEED_> a(A, rows, k, lda);
-        Stream<T, BN, BK_, THREADS, FEED_> b(B, cols, k, ldb);
+        lds_char *const lds = (lds_char *)shared;
         #pragma unroll
         for (int x = 0; x < MB; x++)
             #pragma unroll
-            for (int t = 0; t < 4; t++)
+            for (int t = 0; t < 2; t++)
                 #pragma unroll
                 for (int y = 0; y < NB; y++)
                     #pragma unroll
-                    for (int u = 0; u < 4; u++) acc[x][t][y][u] = Acc{};
-        int const tiles = (k + KT - 1) / KT;
-        if (tiles == 0) return;
-        a.fetch(lds, 0); b.fetch(lds + OA::BYTES, 0);
-        a.put(lds); b.put(lds + OA::BYTES);
-        landed();
-        int now = 0;
-        for (int kt = 0; kt < tiles; kt++) {
-            // (past the last k-tile the fetch reads nothing and leaves zeros)
-            int const next = now ^ STAGE;
-            a.fetch(lds + next, kt + 1); b.fetch(lds + next + OA::BYTES, kt + 1);
-            multiply(lds + now);
-            a.put(lds + next); b.put(lds + next + OA::BYTES);
-            landed();
-            now = next;
+                    for (int u = 0; u < 2; u++) acc[x][t][y][u] = Acc{};
+        int const tiles = tiles_of(p.k);
+        if constexpr (FEED_ == DIRECT) {
+            int const lds0 = __builtin_amdgcn_readfirstlane((int)(unsigned long long)lds);
+            for (int kt = 0; kt < tiles; kt++) {
+                int const place = after(now, 2), ahead = kt + 2 < tiles ? kt + 2 : kt + 2 - tiles;
+                if (kt + 2 == tiles) set_a(next);
+                a.begin(ahead);
+                turn(f[0], f[1], lds + now, lds + after(now, 1), 1, a, lds0 + after(now, 4));
+                // the next k-tile is there, and no wave reads this one's places any more
+                meet<OA::LOADS>();
+                if (kt + 2 == tiles) set_b(next);
+                b.begin(ahead);
+                turn(f[1], f[0], lds + place, lds + after(place, 1), 0, b, lds0 + now);
+                now = place;
+            }
+        } else {
+            if (tiles == 0) return;
+            a.fetch(0, 0); b.fetch(0, 0);
+            a.put(lds, 0); b.put(lds + PLACE, 0);
+            for (int kt = 0; kt < tiles; kt++) {
+                lds_char *const here = lds + (kt & 1) * 2 * PLACE, *const there = lds + (~kt & 1) * 2 * PLACE;
+                meet<0>();
+                a.fetch(0, kt + 1); b.fetch(0, kt + 1);
+                #pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    #pragma unroll
+                    for (int r = 0; r < READS; r++) read(f[0], here, here + PLACE, half, r);
+                    #pragma unroll
+                    for (int q = 0; q < PRODUCTS; q++) multiply(f[0], q);
+                }
+                a.put(there, kt + 1); b.put(there + PLACE, kt + 1);
+            }
         }
     }
 
-    // every wave's part of the next k-tile is in LDS, and every wave is done with this one's
-    static __device__ __forceinline__ void landed()
+    // All tiles of a workgroup: get(turn, plan) makes the plan of its tile number `turn` (false: there is none), done(plan) stores it.
+    template <typename G, typename E>
+    __device__ __forceinline__ void all(char *shared, G &&get, E &&done)
     {
+        Plan<T> p;
+        auto keep = get(0, p);
+        if (!keep.there) return;
+        start(p, shared);
+        for (int turn = 1;; turn++) {
+            Plan<T> next = p;
+            auto const more = get(turn, next);
+            if (!more.there) { next.k = 0; next.rows = next.cols = 0; }
+            next.A = uniform(next.A); next.B = uniform(next.B);
+            next.rows = uniform(next.rows); next.cols = uniform(next.cols); next.k = uniform(next.k); next.r0 = uniform(next.r0); next.c0 = uniform(next.c0);
+            run(p, next, shared);
+            done(p, keep);
+            if (!more.there) break;
+            p = next; keep = more;
+            if constexpr (FEED_ != DIRECT) { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); set_a(p); set_b(p); }
+        }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
     }
 
-    // f(row, column, 16 accumulators of consecutive rows) for every column of the lane's; rows and columns count from the tile's corner
+    // f(row, column, value) for every run of RUN consecutive rows of a column that the lane holds, value(r) its numbers; rows and columns
+    // count from the tile's corner
+    static constexpr int RUN = AK_ ? 8 : 4;
     template <typename F>
     __device__ __forceinline__ void each(F &&f)
     {
-        int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
+        int const lane = thread_now() & 63, wave = wave_number(), j = lane & 31, q = lane >> 5;
         int const m0 = wave % WAVES_M * (BM / WAVES_M), n0 = wave / WAVES_M * (BN / WAVES_N);
         #pragma unroll
         for (int x = 0; x < MB; x++)
             #pragma unroll
             for (int y = 0; y < NB; y++)
                 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    auto const v = [&](int r) { return acc[x][r >> 2][y][u][r & 3]; };
-                    f(m0 + 64 * x + 16 * q, n0 + 64 * y + 16 * (i >> 2) + 4 * u + (i & 3), v);
-                }
+                for (int u = 0; u < 2; u++)
+                    #pragma unroll
+                    for (int g = 0; g < 4; g++)
+                        #pragma unroll
+                        for (int t = 0; t < 8 / RUN; t++) {
+                            auto const v = [&](int r) { return acc[x][AK_ ? r >> 2 : t][y][u][4 * g + (r & 3)]; };
+                            f(m0 + 64 * x + OA::row(8 * g + 4 * q, t), n0 + 64 * y + OB::row(j, u), v);
+                        }
     }
 };
 
-// 16 consecutive numbers of a column, `rows` of which exist; value(r) gives them
-template <typename D, typename V>
-__device__ __forceinline__ void store16(D *to, int rows, bool aligned, V &&value)
+// N consecutive numbers of a column, `rows` of which exist; value(r) gives them.  (Wide stores at any alignment)
+template <int N, typename D, typename V>
+__device__ __forceinline__ void store_run(D *to, int rows, V &&value)
 {
-    constexpr int EL = 16 / (int)sizeof(D);
-    if (rows >= 16 && aligned) {
-        #pragma unroll
-        for (int c = 0; c < 16 / EL; c++) {
-            D one[EL];
-            #pragma unroll
-            for (int e = 0; e < EL; e++) one[e] = (D)value(c * EL + e);
-            i32x4 v;
-            __builtin_memcpy(&v, one, 16);
-            *(i32x4 *)(to + c * EL) = v;
-        }
-        return;
-    }
+    D one[N];
     #pragma unroll
-    for (int r = 0; r < 16; r++)
-        if (r < rows) to[r] = (D)value(r);
+    for (int e = 0; e < N; e++) one[e] = (D)value(e);
+    if (rows >= N) __builtin_memcpy(to, one, sizeof one);
+    else
+        #pragma unroll
+        for (int r = 0; r < N; r++)
+            if (r < rows) to[r] = one[r];
 }
 
 } // namespace sn

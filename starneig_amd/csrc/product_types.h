@@ -8,27 +8,39 @@ namespace sn {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// One matrix instruction multiplies 16 x 64 bytes by 64 bytes x 16: lane l holds the 16 bytes
-// A[i = l & 15][bytes 16 (l >> 4) ...], B[same bytes][j = l & 15] and D[i = 4 (l >> 4) + reg][j = l & 15].
-// The order of the inner index within the 64 bytes is free as long as both operands use the same one.
+// The matrix instructions.  mul: 32 x 32 bytes by 32 bytes x 32, lane l holds the 16 bytes A[i = l & 31][bytes 16 (l >> 5) ...],
+// B[same bytes][j = l & 31] and D[i = 8 (r >> 2) + 4 (l >> 5) + (r & 3)][j = l & 31].  (The products of a 16 x 16 instruction cost the
+// same time, but its operands are read from the registers twice as often: more power, and with it a lower clock.)
+// mul16: 16 x 64 bytes by 64 bytes x 16, the 16 bytes A[i = l & 15][bytes 16 (l >> 4) ...] and D[i = 4 (l >> 4) + r][j = l & 15].
+// The order of the inner index within these bytes is free as long as both operands use the same one.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
 template <typename T> struct Mfma;
 template <> struct Mfma<__bf16> {
-    typedef f32x4 Acc;
+    typedef f32x16 Acc;
+    typedef f32x4 Acc16;
     static __device__ __forceinline__ Acc mul(i32x4 a, i32x4 b, Acc c)
+    { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0); }
+    static __device__ __forceinline__ Acc16 mul16(i32x4 a, i32x4 b, Acc16 c)
     { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0); }
 };
 template <> struct Mfma<_Float16> {
-    typedef f32x4 Acc;
+    typedef f32x16 Acc;
+    typedef f32x4 Acc16;
     static __device__ __forceinline__ Acc mul(i32x4 a, i32x4 b, Acc c)
+    { return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0); }
+    static __device__ __forceinline__ Acc16 mul16(i32x4 a, i32x4 b, Acc16 c)
     { return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0); }
 };
 template <> struct Mfma<signed char> {
-    typedef i32x4 Acc;
-    static __device__ __forceinline__ Acc mul(i32x4 a, i32x4 b, Acc c)
-    { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+    typedef i32x16 Acc;
+    typedef i32x4 Acc16;
+    static __device__ __forceinline__ Acc mul(i32x4 a, i32x4 b, Acc c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Acc16 mul16(i32x4 a, i32x4 b, Acc16 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 };
 
 // The columns [begin, end) of a group, or of the piece of a group that a workgroup takes.
@@ -37,49 +49,59 @@ struct Span { int group, begin, end; };
 // Offsets come from the device (a router's prefix sums) and are not trusted: each is clamped to [0, n] and to its
 // predecessors' maximum, so that the groups are disjoint and inside the matrix whatever the array holds.
 //
-// The groups are cut into pieces of at most `width` columns, in the groups' order; which(number of pieces) names the piece
-// that the caller wants (negative: none).  Every wave walks by itself, 64 groups at a time: a prefix maximum for
-// the offsets and a prefix sum for the pieces, no shared memory and no barrier.
-template <typename F>
-__device__ __forceinline__ Span find_piece(int const *__restrict__ offsets, int groups, int n, int width, F &&which)
-{
-    int const lane = threadIdx.x & 63;
-    int begin, first, count, end, carry, before;
-    auto const start = [&]() { carry = min(max(offsets[0], 0), n); before = 0; };
-    auto const walk = [&](int g0) {
-        int const g = g0 + lane;
-        end = g < groups ? min(max(offsets[g + 1], 0), n) : 0;
+// The groups cut into pieces of at most `width` columns, in the groups' order.  Every wave walks by itself, 64 groups at a time: a prefix
+// maximum for the offsets and a prefix sum for the pieces, no shared memory and no barrier; up to 64 groups
+// stay in the lanes, so that a further piece is found without another walk.
+struct Pieces {
+    int const *offsets;
+    int groups, n, width;
+    int total;                              // pieces
+    int begin, end, first;                  // of the lane's group: its columns, its first piece
+    int carry, before;
+
+    __device__ __forceinline__ Pieces(int const *offsets_, int groups_, int n_, int width_) : offsets(offsets_), groups(groups_), n(n_), width(width_)
+    {
+        start();
+        for (int g0 = 0; g0 < groups; g0 += 64) walk(g0);
+        total = before;
+    }
+    __device__ __forceinline__ int offset(int g) const { return offsets ? min(max(offsets[g], 0), n) : g ? n : 0; }     // (none: one group of all columns)
+    __device__ __forceinline__ void start() { carry = __builtin_amdgcn_readfirstlane(offset(0)); before = 0; }
+    __device__ __forceinline__ void walk(int g0)
+    {
+        int const lane = threadIdx.x & 63, g = g0 + lane;
+        end = g < groups ? offset(g + 1) : 0;
         end = max(end, carry);
         #pragma unroll
         for (int d = 1; d < 64; d *= 2) { int const o = __shfl_up(end, d); if (lane >= d) end = max(end, o); }
         begin = __shfl_up(end, 1);
         if (lane == 0) begin = carry;
-        count = (end - begin + width - 1) / width;
+        int const count = (end - begin + width - 1) / width;
         int sum = count;
         #pragma unroll
         for (int d = 1; d < 64; d *= 2) { int const o = __shfl_up(sum, d); if (lane >= d) sum += o; }
         first = before + sum - count;
         before += __builtin_amdgcn_readlane(sum, 63);
         carry = __builtin_amdgcn_readlane(end, 63);
-    };
-    start();
-    for (int g0 = 0; g0 < groups; g0 += 64) walk(g0);
-    int const piece = which(before);
-    if (piece < 0 || piece >= before) return Span{-1, 0, 0};
-    if (groups > 64) start();
-    for (int g0 = 0;; g0 += 64) {
-        if (groups > 64) walk(g0);
-        unsigned long long const here = __ballot(piece >= first && piece < first + count);
-        if (here) {
-            int const l = __ffsll(here) - 1;
-            Span s;
-            s.group = g0 + l;
-            s.begin = __builtin_amdgcn_readlane(begin, l) + (piece - __builtin_amdgcn_readlane(first, l)) * width;
-            s.end = min(s.begin + width, __builtin_amdgcn_readlane(end, l));
-            return s;
+    }
+    // piece number `piece` < total
+    __device__ __forceinline__ Span at(int piece)
+    {
+        if (groups > 64) start();
+        for (int g0 = 0;; g0 += 64) {
+            if (groups > 64) walk(g0);
+            unsigned long long const here = __ballot(piece >= first && (long)(piece - first) * width < end - begin);
+            if (here) {
+                int const l = __ffsll(here) - 1;
+                Span s;
+                s.group = g0 + l;
+                s.begin = __builtin_amdgcn_readlane(begin, l) + (piece - __builtin_amdgcn_readlane(first, l)) * width;
+                s.end = min(s.begin + width, __builtin_amdgcn_readlane(end, l));
+                return s;
+            }
         }
     }
-}
+};
 
 // The columns of one group.
 __device__ __forceinline__ Span whole_group(int const *__restrict__ offsets, int n, int group)
@@ -103,20 +125,24 @@ static inline long most_pieces(int groups, int n, int width)
     return ((long)n + some * (width - 1)) / width;
 }
 
-// Workgroup `id` of a grid of at least roundup(tiles, 8) workgroups -> tile: workgroups go round the 8 XCDs, and each XCD gets a
-// run of neighbouring tiles, whose operands its own L2 then holds.  Negative: no tile.
-__device__ __forceinline__ long tile_of_workgroup(long tiles)
+// Tile number `turn` of the workgroup, of a grid of a multiple of 8 workgroups: workgroups go round the 8 XCDs, and each XCD gets a
+// run of neighbouring tiles, whose operands its own L2 then holds.  Negative: no more tiles.
+__device__ __forceinline__ int tile_of_workgroup(int tiles, int turn)
 {
-    long const each = (tiles + 7) / 8, at = blockIdx.x >> 3, t = (blockIdx.x & 7) * each + at;
-    return at < each && t < tiles ? t : -1;
+    unsigned const each = ((unsigned)tiles + 7) / 8, at = (blockIdx.x >> 3) + (unsigned)turn * (gridDim.x >> 3), t = (blockIdx.x & 7) * each + at;
+    return at < each && t < (unsigned)tiles ? (int)t : -1;
 }
 // Tiles in bands of 8 tile rows, column by column within the band: the 32 workgroups of an XCD hold 8 + 4 operand panels.
-__device__ __forceinline__ void row_and_column(long t, int rows, int cols, int &row, int &col)
+__device__ __forceinline__ void row_and_column(int t, int rows, int cols, int &row, int &col)
 {
-    long const band = t / (8L * cols), in = t % (8L * cols);
-    int const first = (int)band * 8, high = min(rows - first, 8);
-    row = first + (int)(in % high); col = (int)(in / high);
+    int const band = (unsigned)t / (8u * cols), in = t - band * 8 * cols, first = band * 8, high = min(rows - first, 8);
+    row = first + (unsigned)in % (unsigned)high; col = (unsigned)in / (unsigned)high;
 }
+// the same value in all lanes, in a scalar register
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long uniform(long v)
+{ return (long)((unsigned long)(unsigned)uniform((int)v) | (unsigned long)(unsigned)uniform((int)(v >> 32)) << 32); }
+template <typename P> __device__ __forceinline__ P *uniform(P *p) { return (P *)uniform((long)p); }
 
 // hipLaunchKernel with the error of this launch alone as its result (hipGetLastError would hand out, and clear,
 // an earlier call's).

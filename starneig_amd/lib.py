@@ -512,107 +512,131 @@ def dgemm_device(transA, transB, m, n, k, alpha, tA, ldA, tB, ldB, beta, tC, ldC
 AMD_F64, AMD_F32, AMD_BF16, AMD_F16 = range(4)
 
 
+_product_types = {}
+
+
 def _product_type(t):
-    import torch
-    code = {torch.float64: AMD_F64, torch.float32: AMD_F32, torch.bfloat16: AMD_BF16, torch.float16: AMD_F16}.get(t.dtype)
+    if not _product_types:
+        import torch
+        _product_types.update({torch.float64: AMD_F64, torch.float32: AMD_F32, torch.bfloat16: AMD_BF16, torch.float16: AMD_F16})
+    code = _product_types.get(t.dtype)
     if code is None:
         raise ValueError(f"no product takes {t.dtype}")
     return code
 
 
-def _product_matrix(name, t, *shape, dtype=None):
-    """(pointer, leading dimension, stride of the groups) of a tensor that must have `shape` (None: any size)."""
+def _product_device(t):
+    """(device, its current stream) of a call whose tensors have to be on the current device."""
     import torch
-    if t.dim() != len(shape) or any(s is not None and s != have for s, have in zip(shape, t.shape)):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple('any' if s is None else s for s in shape)}")
-    if dtype is not None and t.dtype != dtype:
+    device = t.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        raise ValueError(f"a tensor is on {t.device}, not on the current device")
+    # (a fortieth of the time of torch.cuda.current_stream(), which is a third of a small call's)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return device, raw(device) if raw else _stream_ptr()
+
+
+def _product_matrix(name, t, shape, dtype, device):
+    """(pointer, leading dimension, stride of the groups) of a tensor of this shape and type on this device."""
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    if t.dtype != dtype:
         raise ValueError(f"{name} is {t.dtype}, not {dtype}")
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, not on the current device")
-    stride = t.stride()
-    if t.numel() and t.shape[-1] > 1 and stride[-1] != 1:
+    rows, stride = shape[-1], t.stride()
+    if stride[-1] != 1 and rows > 1 and t.numel():
         raise ValueError(f"the last dimension of {name} is not contiguous")
-    rows = t.shape[-1]
-    if len(shape) == 1:
+    dims = len(stride)
+    if dims == 1:
         return t.data_ptr(), rows, 0
     # (the stride of a dimension of one entry says nothing)
-    ld = stride[-2] if t.shape[-2] > 1 else max(1, rows)
+    ld = stride[-2] if shape[-2] > 1 else max(1, rows)
     if ld < rows:
         raise ValueError(f"the columns of {name} overlap")
-    return t.data_ptr(), ld, (stride[0] if len(shape) == 3 and t.shape[0] > 1 else 0)
+    return t.data_ptr(), ld, (stride[0] if dims == 3 and shape[0] > 1 else 0)
 
 
-def _product_offsets(t):
+def _product_sizes(name, t):
+    if t.dim() != 2:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not (columns, rows)")
+    return t.shape
+
+
+def _product_offsets(t, device):
     """(pointer, groups) of the groups' first columns, int32, the end of the last group behind them."""
     import torch
     if t.dim() != 1 or t.shape[0] < 2:
         raise ValueError("offsets hold one number more than there are groups, of which there is at least one")
-    if t.shape[0] > 1 and t.stride(0) != 1:
-        raise ValueError("offsets are not contiguous")
-    return _product_matrix("offsets", t, None, dtype=torch.int32)[0], t.shape[0] - 1
+    return _product_matrix("offsets", t, t.shape, torch.int32, device)[0], t.shape[0] - 1
 
 
 def grouped_gemm_device(transA, tOffsets, tA, tB, tC):
     """C_g = op(A_g) B_g: tB (n, k), tC (n, m), tA (groups, m, k) for "T", (groups, k, m) for "N"."""
-    poff, groups = _product_offsets(tOffsets)
-    pb, ldb, _ = _product_matrix("B", tB, None, None)
-    n, k = tB.shape
-    pc, ldc, _ = _product_matrix("C", tC, n, None, dtype=tB.dtype)
-    m = tC.shape[1]
-    pa, lda, stride = _product_matrix("A", tA, groups, *((m, k) if transA in ("T", "t") else (k, m)), dtype=tB.dtype)
+    (device, stream), dtype = _product_device(tB), tB.dtype
+    poff, groups = _product_offsets(tOffsets, device)
+    n, k = _product_sizes("B", tB)
+    m = _product_sizes("C", tC)[1]
+    pb, ldb, _ = _product_matrix("B", tB, (n, k), dtype, device)
+    pc, ldc, _ = _product_matrix("C", tC, (n, m), dtype, device)
+    pa, lda, stride = _product_matrix("A", tA, (groups, m, k) if transA in ("T", "t") else (groups, k, m), dtype, device)
     return load().starneig_amd_grouped_gemm_device(
-        _product_type(tB), transA.encode(), groups, m, n, k, poff, pa, lda, stride, pb, ldb, pc, ldc, _stream_ptr())
+        _product_type(tB), transA.encode(), groups, m, n, k, poff, pa, lda, stride, pb, ldb, pc, ldc, stream)
 
 
 def grouped_outer_device(tOffsets, tX, tY, tD, beta=0.0):
     """D_g = X_g Y_g^T + beta D_g: tX (k, m), tY (k, n), tD (groups, n, m).  With X a layer's inputs and Y the
     gradients of its outputs, D is the gradient of its weights (groups, out, in)."""
-    poff, groups = _product_offsets(tOffsets)
-    px, ldx, _ = _product_matrix("X", tX, None, None)
-    k, m = tX.shape
-    py, ldy, _ = _product_matrix("Y", tY, k, None, dtype=tX.dtype)
-    n = tY.shape[1]
-    pd, ldd, stride = _product_matrix("D", tD, groups, n, m)
+    (device, stream), dtype = _product_device(tX), tX.dtype
+    poff, groups = _product_offsets(tOffsets, device)
+    k, m = _product_sizes("X", tX)
+    n = _product_sizes("Y", tY)[1]
+    px, ldx, _ = _product_matrix("X", tX, (k, m), dtype, device)
+    py, ldy, _ = _product_matrix("Y", tY, (k, n), dtype, device)
+    pd, ldd, stride = _product_matrix("D", tD, (groups, n, m), tD.dtype, device)
     return load().starneig_amd_grouped_outer_device(
-        _product_type(tX), _product_type(tD), groups, m, n, k, poff, px, ldx, py, ldy, beta, pd, ldd, stride, _stream_ptr())
+        _product_type(tX), _product_type(tD), groups, m, n, k, poff, px, ldx, py, ldy, beta, pd, ldd, stride, stream)
 
 
 def quantize_i8_device(tX, tQ, tScale):
     """tQ (n, k) int8 and tScale (n) float32 of tX (n, k): Q = rint(X / scale), scale = max |X| / 127 of the column."""
     import torch
-    px, ldx, _ = _product_matrix("X", tX, None, None)
-    n, k = tX.shape
-    pq, ldq, _ = _product_matrix("Q", tQ, n, k, dtype=torch.int8)
-    ps, _, _ = _product_matrix("scale", tScale, n, dtype=torch.float32)
-    return load().starneig_amd_quantize_i8_device(_product_type(tX), k, n, px, ldx, pq, ldq, ps, _stream_ptr())
+    device, stream = _product_device(tX)
+    n, k = _product_sizes("X", tX)
+    px, ldx, _ = _product_matrix("X", tX, (n, k), tX.dtype, device)
+    pq, ldq, _ = _product_matrix("Q", tQ, (n, k), torch.int8, device)
+    ps, _, _ = _product_matrix("scale", tScale, (n,), torch.float32, device)
+    return load().starneig_amd_quantize_i8_device(_product_type(tX), k, n, px, ldx, pq, ldq, ps, stream)
 
 
 def gemm_i8_device(tA, tScaleA, tB, tScaleB, tC):
     """C = (A^T B) scaled by row and column: tA (m, k) and tB (n, k) int8, tScaleA (m) and tScaleB (n) float32, tC (n, m)."""
     import torch
-    pb, ldb, _ = _product_matrix("B", tB, None, None, dtype=torch.int8)
-    n, k = tB.shape
-    pc, ldc, _ = _product_matrix("C", tC, n, None)
-    m = tC.shape[1]
-    pa, lda, _ = _product_matrix("A", tA, m, k, dtype=torch.int8)
-    psa, _, _ = _product_matrix("scaleA", tScaleA, m, dtype=torch.float32)
-    psb, _, _ = _product_matrix("scaleB", tScaleB, n, dtype=torch.float32)
-    return load().starneig_amd_gemm_i8_device(_product_type(tC), m, n, k, pa, lda, psa, pb, ldb, psb, pc, ldc, _stream_ptr())
+    (device, stream), i8, f32 = _product_device(tB), torch.int8, torch.float32
+    n, k = _product_sizes("B", tB)
+    m = _product_sizes("C", tC)[1]
+    pb, ldb, _ = _product_matrix("B", tB, (n, k), i8, device)
+    pc, ldc, _ = _product_matrix("C", tC, (n, m), tC.dtype, device)
+    pa, lda, _ = _product_matrix("A", tA, (m, k), i8, device)
+    psa, _, _ = _product_matrix("scaleA", tScaleA, (m,), f32, device)
+    psb, _, _ = _product_matrix("scaleB", tScaleB, (n,), f32, device)
+    return load().starneig_amd_gemm_i8_device(_product_type(tC), m, n, k, pa, lda, psa, pb, ldb, psb, pc, ldc, stream)
 
 
 def grouped_gemm_i8_device(tOffsets, tA, tScaleA, tB, tScaleB, tC):
     """The same with tA (groups, m, k) and tScaleA (groups, m) for the columns of every group."""
     import torch
-    poff, groups = _product_offsets(tOffsets)
-    pb, ldb, _ = _product_matrix("B", tB, None, None, dtype=torch.int8)
-    n, k = tB.shape
-    pc, ldc, _ = _product_matrix("C", tC, n, None)
-    m = tC.shape[1]
-    pa, lda, stride = _product_matrix("A", tA, groups, m, k, dtype=torch.int8)
-    psa, ldsa, _ = _product_matrix("scaleA", tScaleA, groups, m, dtype=torch.float32)
-    psb, _, _ = _product_matrix("scaleB", tScaleB, n, dtype=torch.float32)
+    (device, stream), i8, f32 = _product_device(tB), torch.int8, torch.float32
+    poff, groups = _product_offsets(tOffsets, device)
+    n, k = _product_sizes("B", tB)
+    m = _product_sizes("C", tC)[1]
+    pb, ldb, _ = _product_matrix("B", tB, (n, k), i8, device)
+    pc, ldc, _ = _product_matrix("C", tC, (n, m), tC.dtype, device)
+    pa, lda, stride = _product_matrix("A", tA, (groups, m, k), i8, device)
+    psa, ldsa, _ = _product_matrix("scaleA", tScaleA, (groups, m), f32, device)
+    psb, _, _ = _product_matrix("scaleB", tScaleB, (n,), f32, device)
     return load().starneig_amd_grouped_gemm_i8_device(
-        _product_type(tC), groups, m, n, k, poff, pa, lda, stride, psa, ldsa if groups > 1 else 0, pb, ldb, psb, pc, ldc, _stream_ptr())
+        _product_type(tC), groups, m, n, k, poff, pa, lda, stride, psa, ldsa if groups > 1 else 0, pb, ldb, psb, pc, ldc, stream)
 
 
 def lcg_fill_device(t, m, n, seed=2019, mode=0):
