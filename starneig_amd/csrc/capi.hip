@@ -981,12 +981,13 @@ SN_API starneig_error_t starneig_amd_grouped_gemm_device(
 
 SN_API starneig_error_t starneig_amd_grouped_outer_device(
     int type, int typeD, int groups, int m, int n, int k, int const *dOffsets,
-    void const *dX, int ldX, void const *dY, int ldY, double beta, void *dD, int ldD, long strideD, void *stream)
+    void const *dX, int ldX, void const *dY, int ldY, double beta, void *dD, int ldD, long strideD,
+    void *dWork, long workSize, void *stream)
 {
     int const size = product_size(type);
     if (size == 0 || type == STARNEIG_AMD_F32) return -1;
     if (typeD != type && (typeD != STARNEIG_AMD_F32 || type == STARNEIG_AMD_F64)) return -2;
-    if (groups < 1) return -3;
+    if (groups < 1 || groups > 65535) return -3;
     if (m < 0) return -4;
     if (n < 0) return -5;
     if (k < 0) return -6;
@@ -1000,10 +1001,18 @@ SN_API starneig_error_t starneig_amd_grouped_outer_device(
     if (ldD < std::max(1, m)) return -14;
     // (the groups' matrices must not overlap)
     if (some && groups > 1 && strideD < (long)(n - 1) * ldD + m) return -15;
+    if (dWork != NULL && (uintptr_t)dWork % 16 != 0) return -16;
+    if (workSize < 0) return -17;
     if (!g_node.initialized) return STARNEIG_NOT_INITIALIZED;
     if (!some) return STARNEIG_SUCCESS;
     return launched(sn::grouped_outer((hipStream_t)stream, (sn::ProductType)type, (sn::ProductType)typeD, groups, m, n, k, dOffsets,
-        dX, ldX, dY, ldY, beta, dD, ldD, strideD));
+        dX, ldX, dY, ldY, beta, dD, ldD, strideD, dWork, workSize));
+}
+
+SN_API long starneig_amd_grouped_outer_work_size(int type, int groups, int m, int n, int k)
+{
+    if (product_size(type) == 0 || type == STARNEIG_AMD_F32 || groups < 1 || groups > 65535 || m < 1 || n < 1 || k < 1) return 0;
+    return sn::grouped_outer_work_size((sn::ProductType)type, groups, m, n, k);
 }
 
 SN_API starneig_error_t starneig_amd_quantize_i8_device(

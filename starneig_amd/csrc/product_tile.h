@@ -98,7 +98,7 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
     int k;
     unsigned at[O::LOADS];          // byte offsets of the thread's chunks; beyond the buffer where there is nothing to read
 
-    __device__ __forceinline__ void set(T const *base_, int outers, int k_, long ld, int)
+    __device__ __forceinline__ void set(T const *base_, int outers, int k_, long ld)
     {
         base = base_; step = ld * O::KT; k = k_;
         int const thread = thread_now();
@@ -134,8 +134,15 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
         #pragma unroll
         for (int s = 0; s < O::LOADS; s++) load(lds, s);
     }
-    __device__ __forceinline__ void put(lds_char *, int) const {}
+    __device__ __forceinline__ void put(lds_char *, int, int) const {}
 };
+
+// 16 bytes of global memory from any address
+__device__ __forceinline__ i32x4 load16(void const *p)
+{
+    typedef int any_i32x4 __attribute__((ext_vector_type(4), aligned(1)));
+    return *(__attribute__((address_space(1))) any_i32x4 const *)p;
+}
 
 // v moved down by `bits`, zeros from above
 __device__ __forceinline__ i32x4 moved_down(i32x4 v, int bits)
@@ -149,65 +156,40 @@ __device__ __forceinline__ i32x4 moved_down(i32x4 v, int bits)
 }
 
 // Every load is of a whole chunk inside the operand: positions that are not there read others in their place, and a chunk that the end
-// cuts is read from where it ends there.  put() moves such a chunk to its place and zeroes what has to be zero: the
-// inner terms past k.  (Outer positions past the end only meet outputs that are not stored.)  An operand of less than a
-// chunk of contiguous numbers is read number by number.
+// cuts is read from where it ends there (the operand has a chunk of contiguous numbers at least).  put() moves such a chunk to its place and
+// zeroes what has to be zero: the inner terms past k.  (Outer positions past the end only meet outputs that are not stored.)
 template <typename T, int ROWS, bool K, int THREADS>
 struct Stream<T, ROWS, K, THREADS, STAGED> {
     using O = Operand<T, ROWS, K, THREADS>;
     T const *base;
     long ld;
     int outers, k;
-    bool tiny;
-    i32x4 held[O::LOADS];
+    i32x4 held[2][O::LOADS];        // two k-tiles
 
-    // `before`: contiguous positions in front of `base` (MN: the tile's first row)
-    __device__ __forceinline__ void set(T const *base_, int outers_, int k_, long ld_, int before)
-    {
-        base = base_; ld = ld_; outers = outers_; k = k_;
-        tiny = K ? k_ < O::EL : outers_ + before < O::EL;
-    }
+    __device__ __forceinline__ void set(T const *base_, int outers_, int k_, long ld_) { base = base_; ld = ld_; outers = outers_; k = k_; }
 
-    __device__ __forceinline__ void fetch(int, int kt)
+    __device__ __forceinline__ void fetch(int set, int kt)
     {
-        if (kt * O::KT >= k) return;
         #pragma unroll
         for (int s = 0; s < O::LOADS; s++) {
             int outer, inner;
             O::chunk(s * THREADS + threadIdx.x, outer, inner);
             inner += kt * O::KT;
-            if (!tiny) {
-                T const *const p = K ? base + min(outer, outers - 1) * ld + min(inner, k - O::EL)
-                                     : base + min(inner, k - 1) * ld + min(outer, outers - O::EL);
-                __builtin_memcpy(&held[s], p, 16);
-            } else {
-                T const *const p = K ? base + min(outer, outers - 1) * ld : base + min(inner, k - 1) * ld;
-                int const from = K ? inner : outer, end = K ? k : outers;
-                unsigned long long w[2] = {0, 0};
-                #pragma unroll 1
-                for (int e = 0; e < O::EL; e++) {
-                    T const one = p[min(from + e, end - 1)];
-                    unsigned long long bits = 0;
-                    __builtin_memcpy(&bits, &one, sizeof one);
-                    int const at = e * 8 * (int)sizeof(T);
-                    if (from + e < end) w[at >> 6] |= bits << (at & 63);
-                }
-                __builtin_memcpy(&held[s], w, 16);
-            }
+            held[set][s] = load16(K ? base + min(outer, outers - 1) * ld + min(inner, k - O::EL)
+                                    : base + min(inner, k - 1) * ld + min(outer, outers - O::EL));
         }
     }
-    __device__ __forceinline__ void put(lds_char *lds, int kt) const
+    __device__ __forceinline__ void put(lds_char *lds, int set, int kt) const
     {
-        if (kt * O::KT >= k) return;
-        bool const cut = !tiny && (K ? (kt + 1) * O::KT > k : outers < ROWS || (kt + 1) * O::KT > k);
+        bool const cut = (kt + 1) * O::KT > k || (!K && outers < ROWS);
         #pragma unroll
         for (int s = 0; s < O::LOADS; s++) {
-            i32x4 v = held[s];
-            if (cut || (tiny && !K)) {
+            i32x4 v = held[set][s];
+            if (cut) {
                 int outer, inner;
                 O::chunk(s * THREADS + threadIdx.x, outer, inner);
                 inner += kt * O::KT;
-                int const over = tiny ? 0 : K ? inner - (k - O::EL) : outer - (outers - O::EL);
+                int const over = K ? inner - (k - O::EL) : outer - (outers - O::EL);
                 if (over > 0) v = moved_down(v, min(over, O::EL) * 8 * (int)sizeof(T));
                 if (!K && inner >= k) v = (i32x4){0, 0, 0, 0};
             }
@@ -216,8 +198,6 @@ struct Stream<T, ROWS, K, THREADS, STAGED> {
     }
 };
 
-// DIRECT: LDS holds five operands of k-tiles (A, B, A, B, A ... in turn), so that one and a half k-tiles are on their way while one is
-// multiplied.  STAGED: two k-tiles, one in registers on its way.
 // What a tile is the product of.  rows / cols: outputs that exist from its corner on, which is (r0, c0); k: inner terms.
 template <typename T>
 struct Plan {
@@ -274,8 +254,9 @@ struct ProductTile {
         }
     }
     // All but the last LOADS loads of every wave have landed, and every wave has read what it has asked LDS for.
+    // (STAGED: nothing but LDS is waited for; the compiler waits for the registers)
     template <int LOADS>
-    static __device__ __forceinline__ void meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(LOADS) : "memory"); }
+    static __device__ __forceinline__ void meet() { if (FEED_ == STAGED) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(LOADS) : "memory"); }
 
     Stream<T, BM, AK_, THREADS, FEED_> a;
     Stream<T, BN, BK_, THREADS, FEED_> b;
@@ -285,8 +266,8 @@ struct ProductTile {
     // DIRECT: k-tiles of a tile, at least the two that are fetched ahead (what is past k is zero)
     static __device__ __forceinline__ int tiles_of(int k) { int const t = (k + KT - 1) / KT; return FEED_ == DIRECT ? max(t, 2) : t; }
     static __device__ __forceinline__ int after(int place, int n) { place += n * PLACE; return place >= LDS_BYTES ? place - LDS_BYTES : place; }
-    __device__ __forceinline__ void set_a(Plan<T> const &p) { a.set(p.A, p.rows, p.k, p.lda, p.r0); }
-    __device__ __forceinline__ void set_b(Plan<T> const &p) { b.set(p.B, p.cols, p.k, p.ldb, p.c0); }
+    __device__ __forceinline__ void set_a(Plan<T> const &p) { a.set(p.A, p.rows, p.k, p.lda); }
+    __device__ __forceinline__ void set_b(Plan<T> const &p) { b.set(p.B, p.cols, p.k, p.ldb); }
 
     // before the first tile
     __device__ __forceinline__ void start(Plan<T> const &p, char *shared)
@@ -333,19 +314,25 @@ struct ProductTile {
         } else {
             if (tiles == 0) return;
             a.fetch(0, 0); b.fetch(0, 0);
-            a.put(lds, 0); b.put(lds + PLACE, 0);
-            for (int kt = 0; kt < tiles; kt++) {
-                lds_char *const here = lds + (kt & 1) * 2 * PLACE, *const there = lds + (~kt & 1) * 2 * PLACE;
-                meet<0>();
-                a.fetch(0, kt + 1); b.fetch(0, kt + 1);
+            a.fetch(1, 1); b.fetch(1, 1);
+            a.put(lds, 0, 0); b.put(lds + PLACE, 0, 0);
+            for (int kt = 0; kt < tiles; kt += 2) {
                 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    #pragma unroll
-                    for (int r = 0; r < READS; r++) read(f[0], here, here + PLACE, half, r);
-                    #pragma unroll
-                    for (int q = 0; q < PRODUCTS; q++) multiply(f[0], q);
+                for (int p = 0; p < 2; p++) {
+                    lds_char *const here = lds + p * 2 * PLACE, *const there = lds + (p ^ 1) * 2 * PLACE;
+                    meet<0>();
+                    a.fetch(p, kt + p + 2); b.fetch(p, kt + p + 2);
+                    if (kt + p < tiles) {
+                        #pragma unroll
+                        for (int half = 0; half < 2; half++) {
+                            #pragma unroll
+                            for (int r = 0; r < READS; r++) read(f[0], here, here + PLACE, half, r);
+                            #pragma unroll
+                            for (int q = 0; q < PRODUCTS; q++) multiply(f[0], q);
+                        }
+                        a.put(there, p ^ 1, kt + p + 1); b.put(there + PLACE, p ^ 1, kt + p + 1);
+                    }
                 }
-                a.put(there, kt + 1); b.put(there + PLACE, kt + 1);
             }
         }
     }

@@ -117,6 +117,37 @@ __device__ __forceinline__ Span whole_group(int const *__restrict__ offsets, int
     return Span{group, top, end};
 }
 
+// The groups with the longest first (up to 64 groups; more stay in their own order).
+struct Longest {
+    int const *offsets;
+    int groups, n;
+    int begin, end, rank;                   // of the lane's group
+
+    __device__ __forceinline__ Longest(int const *offsets_, int groups_, int n_) : offsets(offsets_), groups(groups_), n(n_)
+    {
+        if (groups > 64) return;
+        int const lane = threadIdx.x & 63;
+        int const before = __builtin_amdgcn_readfirstlane(min(max(offsets[0], 0), n));
+        end = max(lane < groups ? min(max(offsets[lane + 1], 0), n) : 0, before);
+        #pragma unroll
+        for (int d = 1; d < 64; d *= 2) { int const o = __shfl_up(end, d); if (lane >= d) end = max(end, o); }
+        begin = __shfl_up(end, 1);
+        if (lane == 0) begin = before;
+        int const length = end - begin;
+        rank = lane < groups ? 0 : 64;
+        for (int g = 0; g < groups; g++) {
+            int const other = __builtin_amdgcn_readlane(length, g);
+            rank += lane < groups && (other > length || (other == length && g < lane));
+        }
+    }
+    __device__ __forceinline__ Span at(int place)
+    {
+        if (groups > 64) return whole_group(offsets, n, place);
+        int const l = __ffsll((unsigned long long)__ballot(rank == place)) - 1;
+        return Span{l, __builtin_amdgcn_readlane(begin, l), __builtin_amdgcn_readlane(end, l)};
+    }
+};
+
 // The most pieces of `width` columns that `groups` groups of together n columns can have: each group that has a column
 // adds at most width - 1 columns of rounding.
 static inline long most_pieces(int groups, int n, int width)

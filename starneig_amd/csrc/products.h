@@ -13,7 +13,9 @@ hipError_t grouped_gemm(hipStream_t s, ProductType type, bool transA, int groups
     void const *A, int lda, long strideA, void const *B, int ldb, void *C, int ldc);
 // D_g = X_g Y_g^T + beta D_g over the columns of group g; k columns in all
 hipError_t grouped_outer(hipStream_t s, ProductType type, ProductType typeD, int groups, int m, int n, int k, int const *offsets,
-    void const *X, int ldx, void const *Y, int ldy, double beta, void *D, int ldd, long strideD);
+    void const *X, int ldx, void const *Y, int ldy, double beta, void *D, int ldd, long strideD, void *work, long work_size);
+// bytes of `work` with which it is fastest (0: none; with less it runs without)
+long grouped_outer_work_size(ProductType type, int groups, int m, int n, int k);
 // C(r, c) = scaleA_g(r) scaleB(c) sum_i A_g(i, r) B(i, c); offsets NULL: one group of all columns
 hipError_t gemm_i8(hipStream_t s, ProductType typeC, int groups, int m, int n, int k, int const *offsets, signed char const *A, int lda, long strideA,
     float const *scaleA, long strideS, signed char const *B, int ldb, float const *scaleB, void *C, int ldc);

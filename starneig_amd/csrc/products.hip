@@ -4,6 +4,7 @@
 #include "dgemm_tile.h"
 #include "products.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace sn {
 
@@ -35,25 +36,34 @@ void grouped_gemm_kernel(int groups, int m, int n, int k, int const *__restrict_
     });
 }
 
+// One item is a tile of one group over one of `slices` runs of its columns.  The items lie in the order of their lengths, and the workgroups take them
+// to and fro (0 1 2 ... 2 1 0), which evens out what each has to do.  With several slices `out` has a plane of all groups' outputs (m x n without gaps)
+// for each slice, and grouped_outer_sum_kernel adds them up in the slices' order.
 template <typename T, typename D, typename P>
 __global__ __launch_bounds__(P::THREADS, P::PER_SIMD)
-void grouped_outer_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, T const *__restrict__ X, long ldx,
+void grouped_outer_kernel(int groups, int m, int n, int k, int slices, int const *__restrict__ offsets, T const *__restrict__ X, long ldx,
     T const *__restrict__ Y, long ldy, float beta, D *__restrict__ out, long ldd, long strideD)
 {
     __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-    int const rows = (m + P::BM - 1) / P::BM, cols = (n + P::BN - 1) / P::BN;
+    int const rows = (m + P::BM - 1) / P::BM, cols = (n + P::BN - 1) / P::BN, each = rows * cols, items = groups * slices * each;
+    Longest order(offsets, groups, k);
     P tile;
+    struct Place { int group, slice; bool there; };
     tile.all(lds, [&](int turn, Plan<T> &p) {
-        int const t = tile_of_workgroup(groups * rows * cols, turn);
-        if (t < 0) return Place{Span{}, false};
+        int const here = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+        unsigned const i = turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - here : here);
+        if (i >= (unsigned)items) return Place{0, 0, false};
+        Span const s = order.at(i / (unsigned)(each * slices));
+        int const in = i % (unsigned)(each * slices), slice = (unsigned)in / (unsigned)each;
         int row, col;
-        row_and_column((unsigned)t % (unsigned)(rows * cols), rows, cols, row, col);
-        Span const s = whole_group(offsets, k, (unsigned)t / (unsigned)(rows * cols));
+        row_and_column(in - slice * each, rows, cols, row, col);
+        int const length = s.end - s.begin, part = slices == 1 ? length : ((length + slices - 1) / slices + P::KT - 1) / P::KT * P::KT;
+        int const begin = s.begin + (int)min((long)slice * part, (long)length), end = min(begin + part, s.end);
         int const r0 = row * P::BM, c0 = col * P::BN;
-        p = Plan<T>{X + s.begin * ldx + r0, Y + s.begin * ldy + c0, ldx, ldy, m - r0, n - c0, s.end - s.begin, r0, c0};
-        return Place{s, true};
+        p = Plan<T>{X + begin * ldx + r0, Y + begin * ldy + c0, ldx, ldy, m - r0, n - c0, end - begin, r0, c0};
+        return Place{s.group, slice, true};
     }, [&](Plan<T> const &p, Place const &at) {
-        D *const to = out + at.s.group * strideD;
+        D *const to = out + ((long)at.slice * groups + at.group) * strideD;
         tile.each([&](int r, int c, auto &&value) {
             if (p.c0 + c >= n) return;
             D *const d = to + (p.c0 + c) * ldd + p.r0 + r;
@@ -68,6 +78,105 @@ void grouped_outer_kernel(int groups, int m, int n, int k, int const *__restrict
                 store_run<P::RUN>(d, left, value);
         });
     });
+}
+
+template <typename D>
+__global__ __launch_bounds__(256)
+void grouped_outer_sum_kernel(int groups, int m, int n, int slices, float const *__restrict__ planes, float beta, D *__restrict__ out, long ldd, long strideD)
+{
+    long const all = (long)groups * n * m;
+    for (long e = blockIdx.x * 256L + threadIdx.x; e < all; e += gridDim.x * 256L) {
+        float sum = planes[e];
+        for (int s = 1; s < slices; s++) sum += planes[s * all + e];
+        long const column = e / m;
+        D *const to = out + column / n * strideD + column % n * ldd + e % m;
+        *to = (D)(beta == 0.f ? sum : sum + beta * (float)*to);
+    }
+}
+
+// The scaling is three roundings to fp32 and one to the result's type: the empty statement keeps the compiler from fusing the
+// second product with the conversion to fp16, whose one rounding would depend on the type of the result.
+__device__ __forceinline__ float scaled(int sum, float row, float col)
+{
+    float v = (float)sum * row * col;
+    asm("" : "+v"(v));
+    return v;
+}
+
+template <typename D, typename P>
+__global__ __launch_bounds__(P::THREADS, P::PER_SIMD)
+void gemm_i8_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, signed char const *__restrict__ A, long lda, long strideA,
+    float const *__restrict__ scaleA, long strideS, signed char const *__restrict__ B, long ldb, float const *__restrict__ scaleB, D *__restrict__ C, long ldc)
+{
+    __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
+    typedef signed char T;
+    int const rows = (m + P::BM - 1) / P::BM;
+    Pieces pieces(offsets, groups, n, P::BN);
+    P tile;
+    tile.all(lds, [&](int turn, Plan<T> &p) {
+        int const t = tile_of_workgroup(rows * pieces.total, turn);
+        if (t < 0) return Place{Span{}, false};
+        int row, piece;
+        row_and_column(t, rows, pieces.total, row, piece);
+        Span const s = pieces.at(piece);
+        int const r0 = row * P::BM;
+        p = Plan<T>{A + s.group * strideA + r0 * lda, B + s.begin * ldb, lda, ldb, m - r0, s.end - s.begin, k, r0, 0};
+        return Place{s, true};
+    }, [&](Plan<T> const &p, Place const &at) {
+        float const *const sa = scaleA + at.s.group * strideS + p.r0;
+        tile.each([&](int r, int c, auto &&value) {
+            if (at.s.begin + c >= at.s.end) return;
+            float const col = scaleB[at.s.begin + c];
+            int const left = m - p.r0 - r;
+            store_run<P::RUN>(C + (at.s.begin + c) * ldc + p.r0 + r, left, [&](int e) { return scaled(value(e), e < left ? sa[r + e] : 0.f, col); });
+        });
+    });
+}
+
+// Too few contiguous numbers for a 16-byte load (fewer than 8 rows or inner terms of 16 bits, 16 of 8): one wave an output, its lanes
+// stride over the inner index.  Element (r, i) of an operand is at r * rs + i * is.
+template <typename T, typename S>
+__device__ __forceinline__ S narrow_sum(T const *__restrict__ a, long ais, T const *__restrict__ b, long bis, int k)
+{
+    S sum = 0;
+    for (int i = threadIdx.x & 63; i < k; i += 64) sum += (S)a[i * ais] * (S)b[i * bis];
+    #pragma unroll
+    for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
+    return sum;
+}
+
+template <typename T, typename D>
+__global__ __launch_bounds__(256)
+void grouped_gemm_narrow_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, T const *__restrict__ A, long ars, long ais, long strideA,
+    float const *__restrict__ scaleA, long strideS, T const *__restrict__ B, long ldb, float const *__restrict__ scaleB, D *__restrict__ C, long ldc)
+{
+    Pieces pieces(offsets, groups, n, 4);
+    if ((int)blockIdx.x >= pieces.total) return;
+    Span const s = pieces.at(blockIdx.x);
+    int const c = s.begin + (threadIdx.x >> 6);
+    if (c >= s.end) return;
+    for (int r = blockIdx.y; r < m; r += gridDim.y) {
+        T const *const a = A + s.group * strideA + r * ars, *const b = B + c * ldb;
+        D v;
+        if constexpr (sizeof(T) == 1) v = (D)scaled(narrow_sum<T, int>(a, ais, b, 1, k), scaleA[s.group * strideS + r], scaleB[c]);
+        else v = (D)narrow_sum<T, float>(a, ais, b, 1, k);
+        if ((threadIdx.x & 63) == 0) C[c * ldc + r] = v;
+    }
+}
+
+template <typename T, typename D>
+__global__ __launch_bounds__(256)
+void grouped_outer_narrow_kernel(int m, int n, int k, int const *__restrict__ offsets, T const *__restrict__ X, long ldx,
+    T const *__restrict__ Y, long ldy, float beta, D *__restrict__ out, long ldd, long strideD)
+{
+    Span const s = whole_group(offsets, k, blockIdx.z);
+    for (long e = blockIdx.x * 4 + (threadIdx.x >> 6); e < (long)m * n; e += gridDim.x * 4) {
+        long const r = e % m, c = e / m;
+        float v = narrow_sum<T, float>(X + s.begin * ldx + r, ldx, Y + s.begin * ldy + c, ldy, s.end - s.begin);
+        D *const to = out + s.group * strideD + c * ldd + r;
+        if (beta != 0.f) v += beta * (float)*to;
+        if ((threadIdx.x & 63) == 0) *to = (D)v;
+    }
 }
 
 // Few columns a group (a token or a batch of them while text is generated): the matrix is read once, as fast as memory gives it, and nothing
@@ -97,11 +206,11 @@ __device__ __forceinline__ void few_columns_tile(T const *__restrict__ A, long l
     for (; s + U <= min(end, k / (4 * EL)); s += U) {
         i32x4 va[U], vb[U][NT];
         #pragma unroll
-        for (int u = 0; u < U; u++) __builtin_memcpy(&va[u], a + ((s + u) * 4 + q) * EL, 16);
+        for (int u = 0; u < U; u++) va[u] = load16(a + ((s + u) * 4 + q) * EL);
         #pragma unroll
         for (int u = 0; u < U; u++)
             #pragma unroll
-            for (int t = 0; t < NT; t++) __builtin_memcpy(&vb[u][t], b[t] + ((s + u) * 4 + q) * EL, 16);
+            for (int t = 0; t < NT; t++) vb[u][t] = load16(b[t] + ((s + u) * 4 + q) * EL);
         #pragma unroll
         for (int u = 0; u < U; u++)
             #pragma unroll
@@ -112,25 +221,11 @@ __device__ __forceinline__ void few_columns_tile(T const *__restrict__ A, long l
         int skip[U];
         #pragma unroll
         for (int u = 0; u < U; u++) {
-            int const at = ((s + u) * 4 + q) * EL, from = max(min(at, k - EL), 0);
+            int const at = ((s + u) * 4 + q) * EL, from = min(at, k - EL);
             skip[u] = s + u < end ? min(at - from, EL) : EL;
-            if (k >= EL) {
-                __builtin_memcpy(&va[u], a + from, 16);
-                #pragma unroll
-                for (int t = 0; t < NT; t++) __builtin_memcpy(&vb[u][t], b[t] + from, 16);
-            } else {                // (less than one chunk in all: it lies at the chunk's end, as if k cut it)
-                T one[EL];
-                #pragma unroll
-                for (int e = 0; e < EL; e++) one[e] = e < EL - k ? (T)0 : a[e - (EL - k)];
-                __builtin_memcpy(&va[u], one, 16);
-                #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    #pragma unroll
-                    for (int e = 0; e < EL; e++) one[e] = e < EL - k ? (T)0 : b[t][e - (EL - k)];
-                    __builtin_memcpy(&vb[u][t], one, 16);
-                }
-                if (at > 0) skip[u] = EL;
-            }
+            va[u] = load16(a + from);
+            #pragma unroll
+            for (int t = 0; t < NT; t++) vb[u][t] = load16(b[t] + from);
         }
         #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -243,6 +338,7 @@ static hipError_t gemm_tiles(hipStream_t s, int groups, int m, int n, int k, int
     void const *B, int ldb, void *C, int ldc)
 {
     long const tiles = most_pieces(groups, n, P::BN) * ((m + P::BM - 1) / P::BM);
+    if (tiles >= 1L << 31) return hipErrorInvalidConfiguration;
     return launch_kernel(grouped_gemm_kernel<T, P>, dim3(resident<P>(tiles)), P::THREADS, s, 0,
         groups, m, n, k, offsets, (T const *)A, (long)lda, strideA, (T const *)B, (long)ldb, (T *)C, (long)ldc);
 }
@@ -251,13 +347,16 @@ template <typename T, bool TA>
 static hipError_t gemm_launch(hipStream_t s, int groups, int m, int n, int k, int const *offsets, void const *A, int lda, long strideA,
     void const *B, int ldb, void *C, int ldc)
 {
-    if (TA && k > 0 && few_columns(groups, m, n)) {
+    if (TA && k >= 8 && few_columns(groups, m, n)) {
         auto const go = [&](auto kernel, int width) {
             return launch_kernel(kernel, dim3((unsigned)roundup(most_pieces(groups, n, width) * ((m + 15) / 16), 8)), 512, s, 0,
                 groups, m, n, k, offsets, (T const *)A, (long)lda, strideA, (T const *)B, (long)ldb, (T *)C, (long)ldc);
         };
         return go(grouped_gemm_few_kernel<T, 1>, 16);
     }
+    if (k < 8 || (!TA && m < 8))
+        return launch_kernel(grouped_gemm_narrow_kernel<T, T>, dim3((unsigned)most_pieces(groups, n, 4), std::min(m, 65535)), 256, s, 0, groups, m, n, k, offsets,
+            (T const *)A, TA ? (long)lda : 1L, TA ? 1L : (long)lda, strideA, (float const *)nullptr, 0L, (T const *)B, (long)ldb, (float const *)nullptr, (T *)C, (long)ldc);
     bool const fast = direct(A, lda, strideA, TA ? k : m, sizeof(T)) && direct(B, ldb, 0, k, sizeof(T));
     // (the large tile where it leaves no compute unit idle)
     if (most_pieces(groups, n, 256) * ((m + 255) / 256) >= 256)
@@ -276,30 +375,72 @@ hipError_t grouped_gemm(hipStream_t s, ProductType type, bool transA, int groups
     return launch(s, groups, m, n, k, offsets, (double const *)A, lda, strideA, (double const *)B, ldb, (double *)C, ldc);
 }
 
+// What a launch takes, in us: rounds of the workgroups that the chip holds at once, each of so many k-tiles (and what six of them take to begin and
+// to store a tile), plus, cut into slices, writing and reading the planes and a second launch.
+struct Cut { int tile, slices; };
+static double outer_time(Cut c, long groups, long m, long n, long k)
+{
+    long const items = groups * ((m + c.tile - 1) / c.tile) * ((n + c.tile - 1) / c.tile) * c.slices;
+    long const held = c.tile == 256 ? 256 : 512, rounds = (items + held - 1) / held;
+    double const tiles = (double)k / groups / c.slices / 64;
+    return rounds * (tiles + 6) * (c.tile == 256 ? 1.8 : 1.2) + (c.slices > 1 ? 3 + c.slices * (double)groups * m * n * 8 / 4e6 : 0);
+}
+static Cut outer_cut(bool fast, long groups, long m, long n, long k)
+{
+    Cut best = {128, 1};
+    for (int tile : {256, 128})
+        for (int slices : {1, 2, 4, 8, 16, 32, 64}) {
+            Cut const c = {tile, slices};
+            if ((tile == 256 && !fast) || (slices > 1 && k / groups / slices < 64)) continue;
+            if (outer_time(c, groups, m, n, k) < outer_time(best, groups, m, n, k)) best = c;
+        }
+    return best;
+}
+
 template <typename T, typename D, typename P>
-static hipError_t outer_tiles(hipStream_t s, int groups, int m, int n, int k, int const *offsets, void const *X, int ldx, void const *Y, int ldy,
+static hipError_t outer_tiles(hipStream_t s, int slices, int groups, int m, int n, int k, int const *offsets, void const *X, int ldx, void const *Y, int ldy,
     double beta, void *out, int ldd, long strideD)
 {
-    long const tiles = (long)groups * ((m + P::BM - 1) / P::BM) * ((n + P::BN - 1) / P::BN);
-    return launch_kernel(grouped_outer_kernel<T, D, P>, dim3((unsigned)roundup(tiles, 8)), P::THREADS, s, 0,
-        groups, m, n, k, offsets, (T const *)X, (long)ldx, (T const *)Y, (long)ldy, (float)beta, (D *)out, (long)ldd, strideD);
+    long const items = (long)groups * slices * ((m + P::BM - 1) / P::BM) * ((n + P::BN - 1) / P::BN);
+    if (items >= 1L << 31) return hipErrorInvalidConfiguration;
+    return launch_kernel(grouped_outer_kernel<T, D, P>, dim3(resident<P>(items)), P::THREADS, s, 0,
+        groups, m, n, k, slices, offsets, (T const *)X, (long)ldx, (T const *)Y, (long)ldy, (float)beta, (D *)out, (long)ldd, strideD);
 }
 
 template <typename T, typename D>
 static hipError_t outer_launch(hipStream_t s, int groups, int m, int n, int k, int const *offsets, void const *X, int ldx, void const *Y, int ldy,
-    double beta, void *out, int ldd, long strideD)
+    double beta, void *out, int ldd, long strideD, void *work, long work_size)
 {
+    if (m < 8 || n < 8)
+        return launch_kernel(grouped_outer_narrow_kernel<T, D>, dim3((unsigned)std::min((long)m * n / 4 + 1, 16384L), 1, groups), 256, s, 0,
+            m, n, k, offsets, (T const *)X, (long)ldx, (T const *)Y, (long)ldy, (float)beta, (D *)out, (long)ldd, strideD);
     bool const fast = direct(X, ldx, 0, m, sizeof(T)) && direct(Y, ldy, 0, n, sizeof(T));
-    // (the large tile where it leaves no compute unit idle)
-    if ((long)groups * ((m + 255) / 256) * ((n + 255) / 256) >= 256)
-    return (fast ? outer_tiles<T, D, ProductTile<T, 256, 256, 2, 4, false, false, DIRECT>> : outer_tiles<T, D, ProductTile<T, 128, 128, 2, 2, false, false, STAGED>>)
-        (s, groups, m, n, k, offsets, X, ldx, Y, ldy, beta, out, ldd, strideD);
-    return (fast ? outer_tiles<T, D, ProductTile<T, 128, 128, 2, 2, false, false, DIRECT>> : outer_tiles<T, D, ProductTile<T, 128, 128, 2, 2, false, false, STAGED>>)
-        (s, groups, m, n, k, offsets, X, ldx, Y, ldy, beta, out, ldd, strideD);
+    Cut c = outer_cut(fast, groups, m, n, k);
+    long const plane = (long)groups * m * n * 4;
+    if (c.slices > 1 && (work == nullptr || work_size < c.slices * plane)) c.slices = 1;
+    auto const go = [&](auto *to, int ld, long stride, double b) {
+        typedef std::remove_pointer_t<decltype(to)> O;
+        auto const launch = c.tile == 256 ? outer_tiles<T, O, ProductTile<T, 256, 256, 2, 4, false, false, DIRECT>>
+            : fast ? outer_tiles<T, O, ProductTile<T, 128, 128, 2, 2, false, false, DIRECT>> : outer_tiles<T, O, ProductTile<T, 128, 128, 2, 2, false, false, STAGED>>;
+        return launch(s, c.slices, groups, m, n, k, offsets, X, ldx, Y, ldy, b, to, ld, stride);
+    };
+    if (c.slices == 1) return go((D *)out, ldd, strideD, beta);
+    hipError_t const e = go((float *)work, m, (long)m * n, 0.0);
+    if (e != hipSuccess) return e;
+    return launch_kernel(grouped_outer_sum_kernel<D>, dim3((unsigned)std::min(((long)groups * m * n + 255) / 256, 4096L)), 256, s, 0,
+        groups, m, n, c.slices, (float const *)work, (float)beta, (D *)out, (long)ldd, strideD);
+}
+
+long grouped_outer_work_size(ProductType type, int groups, int m, int n, int k)
+{
+    if (type == PRODUCT_F64 || m < 8 || n < 8) return 0;
+    // (whichever way the operands are aligned)
+    int const slices = std::max(outer_cut(true, groups, m, n, k).slices, outer_cut(false, groups, m, n, k).slices);
+    return slices > 1 ? (long)slices * groups * m * n * 4 : 0;
 }
 
 hipError_t grouped_outer(hipStream_t s, ProductType type, ProductType typeD, int groups, int m, int n, int k, int const *offsets,
-    void const *X, int ldx, void const *Y, int ldy, double beta, void *D, int ldd, long strideD)
+    void const *X, int ldx, void const *Y, int ldy, double beta, void *D, int ldd, long strideD, void *work, long work_size)
 {
     if (type == PRODUCT_F64)
         return launch_kernel(grouped_douter_kernel, dim3((m + 63) / 64, (n + 63) / 64, groups), 256, s, GemmCfg<64, 64, 16, false, true>::LDS_BYTES,
@@ -307,49 +448,10 @@ hipError_t grouped_outer(hipStream_t s, ProductType type, ProductType typeD, int
     bool const wide = typeD == PRODUCT_F32;
     auto const launch = type == PRODUCT_BF16 ? (wide ? outer_launch<__bf16, float> : outer_launch<__bf16, __bf16>)
                                              : (wide ? outer_launch<_Float16, float> : outer_launch<_Float16, _Float16>);
-    return launch(s, groups, m, n, k, offsets, X, ldx, Y, ldy, beta, D, ldd, strideD);
+    return launch(s, groups, m, n, k, offsets, X, ldx, Y, ldy, beta, D, ldd, strideD, work, work_size);
 }
 
 // ---- 8-bit integers ----------------------------------------------------------------------------------------------
-
-// The scaling is three roundings to fp32 and one to the result's type: the empty statement keeps the compiler from fusing the
-// second product with the conversion to fp16, whose one rounding would depend on the type of the result.
-__device__ __forceinline__ float scaled(int sum, float row, float col)
-{
-    float v = (float)sum * row * col;
-    asm("" : "+v"(v));
-    return v;
-}
-
-template <typename D, typename P>
-__global__ __launch_bounds__(P::THREADS, P::PER_SIMD)
-void gemm_i8_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, signed char const *__restrict__ A, long lda, long strideA,
-    float const *__restrict__ scaleA, long strideS, signed char const *__restrict__ B, long ldb, float const *__restrict__ scaleB, D *__restrict__ C, long ldc)
-{
-    __shared__ __attribute__((aligned(16))) char lds[P::LDS_BYTES];
-    typedef signed char T;
-    int const rows = (m + P::BM - 1) / P::BM;
-    Pieces pieces(offsets, groups, n, P::BN);
-    P tile;
-    tile.all(lds, [&](int turn, Plan<T> &p) {
-        int const t = tile_of_workgroup(rows * pieces.total, turn);
-        if (t < 0) return Place{Span{}, false};
-        int row, piece;
-        row_and_column(t, rows, pieces.total, row, piece);
-        Span const s = pieces.at(piece);
-        int const r0 = row * P::BM;
-        p = Plan<T>{A + s.group * strideA + r0 * lda, B + s.begin * ldb, lda, ldb, m - r0, s.end - s.begin, k, r0, 0};
-        return Place{s, true};
-    }, [&](Plan<T> const &p, Place const &at) {
-        float const *const sa = scaleA + at.s.group * strideS + p.r0;
-        tile.each([&](int r, int c, auto &&value) {
-            if (at.s.begin + c >= at.s.end) return;
-            float const col = scaleB[at.s.begin + c];
-            int const left = m - p.r0 - r;
-            store_run<P::RUN>(C + (at.s.begin + c) * ldc + p.r0 + r, left, [&](int e) { return scaled(value(e), e < left ? sa[r + e] : 0.f, col); });
-        });
-    });
-}
 
 template <typename D, int NT>
 __global__ __launch_bounds__(512)
@@ -372,6 +474,7 @@ static hipError_t gemm_i8_tiles(hipStream_t s, int groups, int m, int n, int k, 
     float const *scaleA, long strideS, signed char const *B, int ldb, float const *scaleB, void *C, int ldc)
 {
     long const tiles = most_pieces(groups, n, P::BN) * ((m + P::BM - 1) / P::BM);
+    if (tiles >= 1L << 31) return hipErrorInvalidConfiguration;
     return launch_kernel(gemm_i8_kernel<D, P>, dim3(resident<P>(tiles)), P::THREADS, s, 0,
         groups, m, n, k, offsets, A, (long)lda, strideA, scaleA, strideS, B, (long)ldb, scaleB, (D *)C, (long)ldc);
 }
@@ -380,13 +483,16 @@ template <typename D>
 static hipError_t gemm_i8_launch(hipStream_t s, int groups, int m, int n, int k, int const *offsets, signed char const *A, int lda, long strideA,
     float const *scaleA, long strideS, signed char const *B, int ldb, float const *scaleB, void *C, int ldc)
 {
-    if (k > 0 && few_columns(groups, m, n)) {
+    if (k >= 16 && few_columns(groups, m, n)) {
         auto const go = [&](auto kernel, int width) {
             return launch_kernel(kernel, dim3((unsigned)roundup(most_pieces(groups, n, width) * ((m + 15) / 16), 8)), 512, s, 0,
                 groups, m, n, k, offsets, A, (long)lda, strideA, scaleA, strideS, B, (long)ldb, scaleB, (D *)C, (long)ldc);
         };
         return go(gemm_i8_few_kernel<D, 1>, 16);
     }
+    if (k < 16)
+        return launch_kernel(grouped_gemm_narrow_kernel<signed char, D>, dim3((unsigned)most_pieces(groups, n, 4), std::min(m, 65535)), 256, s, 0, groups, m, n, k, offsets,
+            A, (long)lda, 1L, strideA, scaleA, strideS, B, (long)ldb, scaleB, (D *)C, (long)ldc);
     bool const fast = direct(A, lda, strideA, k, 1) && direct(B, ldb, 0, k, 1);
     typedef signed char T;
     // (the large tile where it leaves no compute unit idle)

@@ -125,7 +125,8 @@ SIGNATURES = {
                   _vp, C.c_int, _vp, C.c_int, _vp]),
     "starneig_amd_grouped_outer_device": (
         C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp, C.c_int, _vp, C.c_int,
-                  C.c_double, _vp, C.c_int, C.c_long, _vp]),
+                  C.c_double, _vp, C.c_int, C.c_long, _vp, C.c_long, _vp]),
+    "starneig_amd_grouped_outer_work_size": (C.c_long, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     "starneig_amd_quantize_i8_device": (
         C.c_int, [C.c_int, C.c_int, C.c_int, _vp, C.c_int, _vp, C.c_int, _vp, _vp]),
     "starneig_amd_gemm_i8_device": (
@@ -586,16 +587,22 @@ def grouped_gemm_device(transA, tOffsets, tA, tB, tC):
 
 def grouped_outer_device(tOffsets, tX, tY, tD, beta=0.0):
     """D_g = X_g Y_g^T + beta D_g: tX (k, m), tY (k, n), tD (groups, n, m).  With X a layer's inputs and Y the
-    gradients of its outputs, D is the gradient of its weights (groups, out, in)."""
+    gradients of its outputs, D is the gradient of its weights (groups, out, in).  The scratch memory is the
+    caching allocator's, on the current stream."""
+    import torch
     (device, stream), dtype = _product_device(tX), tX.dtype
     poff, groups = _product_offsets(tOffsets, device)
     k, m = _product_sizes("X", tX)
     n = _product_sizes("Y", tY)[1]
     px, ldx, _ = _product_matrix("X", tX, (k, m), dtype, device)
     py, ldy, _ = _product_matrix("Y", tY, (k, n), dtype, device)
-    pd, ldd, stride = _product_matrix("D", tD, (groups, n, m), tD.dtype, device)
-    return load().starneig_amd_grouped_outer_device(
-        _product_type(tX), _product_type(tD), groups, m, n, k, poff, px, ldx, py, ldy, beta, pd, ldd, stride, stream)
+    pd, ldd, strided = _product_matrix("D", tD, (groups, n, m), tD.dtype, device)
+    lib, code = load(), _product_type(tX)
+    size = lib.starneig_amd_grouped_outer_work_size(code, groups, m, n, k)
+    work = torch.empty(size, dtype=torch.uint8, device=tX.device) if size else None
+    return lib.starneig_amd_grouped_outer_device(
+        code, _product_type(tD), groups, m, n, k, poff, px, ldx, py, ldy, beta, pd, ldd, strided,
+        work.data_ptr() if size else None, size, stream)
 
 
 def quantize_i8_device(tX, tQ, tScale):

@@ -14,7 +14,7 @@ def call(name, args, **change):
 
 
 GEMM = dict(type=S.AMD_BF16, trans=b"T", groups=2, m=8, n=6, k=16, off=P, A=P, ldA=16, strideA=128, B=P, ldB=16, C=P, ldC=8, stream=None)
-OUTER = dict(type=S.AMD_F16, typeD=S.AMD_F32, groups=2, m=8, n=6, k=16, off=P, X=P, ldX=8, Y=P, ldY=6, beta=0.0, D=P, ldD=8, strideD=48, stream=None)
+OUTER = dict(type=S.AMD_F16, typeD=S.AMD_F32, groups=2, m=8, n=6, k=16, off=P, X=P, ldX=8, Y=P, ldY=6, beta=0.0, D=P, ldD=8, strideD=48, work=None, workSize=0, stream=None)
 QUANT = dict(type=S.AMD_F32, k=16, n=3, X=P, ldX=16, Q=P, ldQ=16, scale=P, stream=None)
 I8 = dict(typeC=S.AMD_BF16, m=8, n=6, k=16, A=P, ldA=16, sA=P, B=P, ldB=16, sB=P, C=P, ldC=8, stream=None)
 GI8 = dict(typeC=S.AMD_F16, groups=2, m=8, n=6, k=16, off=P, A=P, ldA=16, strideA=128, sA=P, strideS=8, B=P, ldB=16, sB=P, C=P, ldC=8, stream=None)
@@ -27,7 +27,7 @@ REFUSED = [
     ("grouped_outer_device", OUTER, [
         (1, dict(type=S.AMD_F32)), (2, dict(typeD=S.AMD_BF16)), (2, dict(typeD=S.AMD_F64)), (2, dict(type=S.AMD_F64)), (3, dict(groups=0)), (4, dict(m=-1)),
         (5, dict(n=-1)), (6, dict(k=-1)), (7, dict(off=None)), (8, dict(X=None)), (9, dict(ldX=7)), (10, dict(Y=None)), (11, dict(ldY=5)),
-        (13, dict(D=None)), (13, dict(D=P + 2)), (14, dict(ldD=7)), (15, dict(strideD=47)), (15, dict(strideD=0))]),
+        (13, dict(D=None)), (13, dict(D=P + 2)), (14, dict(ldD=7)), (3, dict(groups=65536)), (15, dict(strideD=47)), (15, dict(strideD=0)), (16, dict(work=P + 8)), (17, dict(work=P, workSize=-1))]),
     ("quantize_i8_device", QUANT, [
         (1, dict(type=S.AMD_F64)), (1, dict(type=4)), (2, dict(k=-1)), (3, dict(n=-1)), (4, dict(X=None)), (4, dict(X=P + 2)), (5, dict(ldX=15)),
         (6, dict(Q=None)), (7, dict(ldQ=15)), (8, dict(scale=None)), (8, dict(scale=P + 1))]),
@@ -70,3 +70,13 @@ def test_binding_refuses_host_tensors_and_shapes():
         S.grouped_gemm_device("T", off[:1], x, x, x)
     with pytest.raises(ValueError):
         S.quantize_i8_device(x, torch.zeros(4, 7, dtype=torch.int8), torch.zeros(4))
+
+
+def test_work_size():
+    size = S.lib.load().starneig_amd_grouped_outer_work_size
+    assert size(S.AMD_BF16, 1, 512, 384, 20000) % (512 * 384 * 4) == 0 and size(S.AMD_BF16, 1, 512, 384, 20000) > 0      # few outputs, a long sum
+    assert size(S.AMD_F16, 16, 4096, 2048, 32768) == 0              # outputs enough
+    assert size(S.AMD_F64, 1, 512, 384, 20000) == 0
+    for refused in [(S.AMD_F32, 1, 512, 384, 20000), (9, 1, 512, 384, 20000), (S.AMD_BF16, 0, 512, 384, 20000), (S.AMD_BF16, 65536, 512, 384, 20000),
+                    (S.AMD_BF16, 1, 0, 384, 20000), (S.AMD_BF16, 1, 512, -1, 20000), (S.AMD_BF16, 1, 512, 384, 0)]:
+        assert size(*refused) == 0
