@@ -40,8 +40,10 @@ __device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, int t
 }
 // threadIdx.x for what is computed once a tile: the compiler must not compute it before the loops and hold it in registers meanwhile
 __device__ __forceinline__ int thread_now() { int t = threadIdx.x; asm volatile("" : "+v"(t)); return t; }
+// number of the wave, of the threads that share a tile
 __device__ __forceinline__ int wave_number() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
+// THREADS: how many bring the operand together, the workgroup's or a wave's
 template <typename T, int ROWS, bool K, int THREADS>
 struct Operand {
     static constexpr int EL = 16 / (int)sizeof(T);          // numbers a chunk
@@ -52,7 +54,7 @@ struct Operand {
 
     // (ds_read_b128 serves 16 lanes at a time: 0-3, 12-15, 20-27; 4-11, 16-19, 28-31; and so on; ds_read_b64_tr_b16 32)
     static __device__ __forceinline__ int swizzle_k(int r) { return (r >> 1 & 1) | (r >> 3 & 6); }
-    static __device__ __forceinline__ int swizzle_mn(int k) { return (k & 3) << 2; }
+    static __device__ __forceinline__ int swizzle_mn(int k) { return CR >= 16 ? (k & 3) << 2 : (k & 2) << 1; }
 
     // row of lane i of fragment t of 64 rows
     static __device__ __forceinline__ int row(int i, int t) { return K ? 8 * (i >> 2) + 4 * t + (i & 3) : 32 * t + i; }
@@ -101,7 +103,7 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
     __device__ __forceinline__ void set(T const *base_, int outers, int k_, long ld)
     {
         base = base_; step = ld * O::KT; k = k_;
-        int const thread = thread_now();
+        int const thread = thread_now() % THREADS;
         #pragma unroll
         for (int s = 0; s < O::LOADS; s++) {
             int outer, in;
@@ -117,7 +119,7 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
     {
         int const left = k - kt * O::KT;
         if (left < O::KT && left > 0) {
-            int const thread = thread_now();
+            int const thread = thread_now() % THREADS;
             #pragma unroll
             for (int s = 0; s < O::LOADS; s++) {
                 int outer, inner;
@@ -127,7 +129,7 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
         }
         from = buffer(K ? base + (long)kt * O::KT : base + kt * step, left > 0 ? 0x7fffffff : 0);
     }
-    __device__ __forceinline__ void load(int lds, int s) const { load_to_lds(from, at[s], lds + wave_number() * 1024 + s * THREADS * 16); }
+    __device__ __forceinline__ void load(int lds, int s) const { load_to_lds(from, at[s], lds + wave_number() % (THREADS / 64) * 1024 + s * THREADS * 16); }
     __device__ __forceinline__ void fetch(int lds, int kt)
     {
         begin(kt);
@@ -173,7 +175,7 @@ struct Stream<T, ROWS, K, THREADS, STAGED> {
         #pragma unroll
         for (int s = 0; s < O::LOADS; s++) {
             int outer, inner;
-            O::chunk(s * THREADS + threadIdx.x, outer, inner);
+            O::chunk(s * THREADS + (int)threadIdx.x % THREADS, outer, inner);
             inner += kt * O::KT;
             held[set][s] = load16(K ? base + min(outer, outers - 1) * ld + min(inner, k - O::EL)
                                     : base + min(inner, k - 1) * ld + min(outer, outers - O::EL));
@@ -187,13 +189,13 @@ struct Stream<T, ROWS, K, THREADS, STAGED> {
             i32x4 v = held[set][s];
             if (cut) {
                 int outer, inner;
-                O::chunk(s * THREADS + threadIdx.x, outer, inner);
+                O::chunk(s * THREADS + (int)threadIdx.x % THREADS, outer, inner);
                 inner += kt * O::KT;
                 int const over = K ? inner - (k - O::EL) : outer - (outers - O::EL);
                 if (over > 0) v = moved_down(v, min(over, O::EL) * 8 * (int)sizeof(T));
                 if (!K && inner >= k) v = (i32x4){0, 0, 0, 0};
             }
-            *(lds_i32x4 *)(lds + (s * THREADS + threadIdx.x) * 16) = v;
+            *(lds_i32x4 *)(lds + (s * THREADS + (int)threadIdx.x % THREADS) * 16) = v;
         }
     }
 };
@@ -206,18 +208,20 @@ struct Plan {
     int rows, cols, k, r0, c0;
 };
 
-template <typename T, int BM_, int BN_, int WAVES_M_, int WAVES_N_, bool AK_, bool BK_, Feed FEED_>
+// WAVES_K > 1: so many waves, each by itself, with a part of the inner index and of LDS; their sums are added up in their order.
+template <typename T, int BM_, int BN_, int WAVES_M_, int WAVES_N_, bool AK_, bool BK_, Feed FEED_, int WAVES_K_ = 1>
 struct ProductTile {
-    static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, THREADS = 64 * WAVES_M * WAVES_N;
+    static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, WAVES_K = WAVES_K_, SHARE = 64 * WAVES_M * WAVES_N, THREADS = SHARE * WAVES_K;
+    static_assert(WAVES_K == 1 || SHARE == 64, "each wave by itself");
     static constexpr int MB = BM / WAVES_M / 64, NB = BN / WAVES_N / 64;     // 64 x 64 blocks a wave
     static_assert(BM == BN, "the places in LDS are of one size");
     typedef typename Mfma<T>::Acc Acc;
-    using OA = Operand<T, BM, AK_, THREADS>;
-    using OB = Operand<T, BN, BK_, THREADS>;
-    static constexpr int PLACE = OA::BYTES, PLACES = FEED_ == DIRECT ? 5 : 4, LDS_BYTES = PLACES * PLACE;
+    using OA = Operand<T, BM, AK_, SHARE>;
+    using OB = Operand<T, BN, BK_, SHARE>;
+    static constexpr int PLACE = OA::BYTES, PLACES = FEED_ == DIRECT ? 5 : 4, RING = PLACES * PLACE, LDS_BYTES = RING * WAVES_K;
     static constexpr int KT = OA::KT;
     static constexpr bool A_K = AK_;
-    static constexpr int PER_SIMD = MB * NB > 2 ? 1 : 2;        // waves
+    static constexpr int PER_SIMD = MB * NB > 2 || WAVES_K > 1 ? 1 : 2;     // waves
 
     Acc acc[MB][2][NB][2];
 
@@ -227,7 +231,7 @@ struct ProductTile {
     static constexpr int READS = 4 * (MB + NB), PRODUCTS = 8 * MB * NB;         // of half a k-tile
     static __device__ __forceinline__ void read(Fragments &f, lds_char const *la, lds_char const *lb, int half, int r)
     {
-        int const wave = wave_number(), m0 = wave % WAVES_M * (BM / WAVES_M), n0 = wave / WAVES_M * (BN / WAVES_N);
+        int const wave = wave_number() % (SHARE / 64), m0 = wave % WAVES_M * (BM / WAVES_M), n0 = wave / WAVES_M * (BN / WAVES_N);
         int const s = r / (2 * (MB + NB)), i = r % (2 * (MB + NB)), x = i / 2 - NB, y = i / 2, t = i % 2;
         if (y < NB) f.b[s][y][t] = OB::fragment(lb, n0 + 64 * y, t, 2 * half + s);
         else        f.a[s][x][t] = OA::fragment(la, m0 + 64 * x, t, 2 * half + s);
@@ -242,30 +246,37 @@ struct ProductTile {
     template <typename S>
     __device__ __forceinline__ void turn(Fragments const &f, Fragments &g, lds_char const *la, lds_char const *lb, int half, S &stream, int place)
     {
-        constexpr int LOADS = S::O::LOADS, LAST = PRODUCTS - (PRODUCTS >= 16 ? 6 : 2);       // the reads early: the next turn begins with what they bring
+        constexpr int LOADS = S::O::LOADS;
         #pragma unroll
         for (int p = 0; p < PRODUCTS; p++) {
             #pragma unroll
-            for (int r = 0; r < READS; r++) if (r * LAST / READS == p) read(g, la, lb, half, r);
+            for (int r = 0; r < READS; r++) if (r * PRODUCTS / READS == p) read(g, la, lb, half, r);
+            if (p == 0) __builtin_amdgcn_s_setprio(1);
             multiply(f, p);
             #pragma unroll
             for (int l = 0; l < LOADS; l++) if ((2 * l + 1) * PRODUCTS / (2 * LOADS) == p) stream.load(place, l);
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
     }
     // All but the last LOADS loads of every wave have landed, and every wave has read what it has asked LDS for.
-    // (STAGED: nothing but LDS is waited for; the compiler waits for the registers)
+    // (STAGED: nothing but LDS is waited for; the compiler waits for the registers.  A wave by itself meets nobody.)
     template <int LOADS>
-    static __device__ __forceinline__ void meet() { if (FEED_ == STAGED) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(LOADS) : "memory"); }
+    static __device__ __forceinline__ void meet()
+    {
+        if constexpr (FEED_ == STAGED) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(LOADS) : "memory");
+        if constexpr (WAVES_K == 1) asm volatile("s_barrier" ::: "memory");
+    }
 
-    Stream<T, BM, AK_, THREADS, FEED_> a;
-    Stream<T, BN, BK_, THREADS, FEED_> b;
+    Stream<T, BM, AK_, SHARE, FEED_> a;
+    Stream<T, BN, BK_, SHARE, FEED_> b;
     Fragments f[FEED_ == DIRECT ? 2 : 1];
     int now;
 
     // DIRECT: k-tiles of a tile, at least the two that are fetched ahead (what is past k is zero)
     static __device__ __forceinline__ int tiles_of(int k) { int const t = (k + KT - 1) / KT; return FEED_ == DIRECT ? max(t, 2) : t; }
-    static __device__ __forceinline__ int after(int place, int n) { place += n * PLACE; return place >= LDS_BYTES ? place - LDS_BYTES : place; }
+    static __device__ __forceinline__ int after(int place, int n) { place += n * PLACE; return place >= RING ? place - RING : place; }
     __device__ __forceinline__ void set_a(Plan<T> const &p) { a.set(p.A, p.rows, p.k, p.lda); }
     __device__ __forceinline__ void set_b(Plan<T> const &p) { b.set(p.B, p.cols, p.k, p.ldb); }
 
@@ -337,13 +348,30 @@ struct ProductTile {
         }
     }
 
-    // All tiles of a workgroup: get(turn, plan) makes the plan of its tile number `turn` (false: there is none), done(plan) stores it.
+    // All tiles of a workgroup: get(turn, plan) makes the plan of its tile number `turn` (`there` false: there is none), done(plan, what get gave)
+    // stores it.  WAVES_K > 1: one tile.
     template <typename G, typename E>
     __device__ __forceinline__ void all(char *shared, G &&get, E &&done)
     {
         Plan<T> p;
         auto keep = get(0, p);
         if (!keep.there) return;
+        if constexpr (WAVES_K > 1) {
+            Plan<T> mine = p;
+            int const part = ((p.k + KT - 1) / KT + WAVES_K - 1) / WAVES_K * KT, k0 = min(wave_number() * part, p.k);
+            mine.A = uniform(p.A + k0 * (AK_ ? 1L : p.lda)); mine.B = uniform(p.B + k0 * (BK_ ? 1L : p.ldb));
+            mine.k = uniform(min(part, p.k - k0));
+            Plan<T> none = mine;
+            none.k = 0; none.rows = none.cols = 0;
+            char *const ring = shared + wave_number() * RING;
+            // (STAGED: the chunk that k cuts is read from where it ends there, in front of the part if that is shorter)
+            start(mine, ring);
+            run(mine, none, ring);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            add_up((lds_char *)shared);
+            done(p, keep);
+            return;
+        }
         start(p, shared);
         for (int turn = 1;; turn++) {
             Plan<T> next = p;
@@ -360,13 +388,39 @@ struct ProductTile {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 
+    // WAVES_K = 4: wave w is left with the sums of registers 4 w ... 4 w + 3 of every accumulator, in registers 0 ... 3
+    __device__ __forceinline__ void add_up(lds_char *lds)
+    {
+        static_assert(WAVES_K == 1 || (WAVES_K == 4 && MB == 1 && NB == 1), "four times four registers");
+        typedef typename Mfma<T>::Acc16 Four;
+        typedef __attribute__((address_space(3))) Four lds_four;
+        lds_four *const all = (lds_four *)lds;          // [wave that summed][wave that takes][2 t + u][lane]
+        int const lane = threadIdx.x & 63, wave = wave_number();
+        #pragma unroll
+        for (int g = 0; g < 4; g++)
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                auto const &v = acc[0][i >> 1][0][i & 1];
+                all[((wave * 4 + g) * 4 + i) * 64 + lane] = Four{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+            }
+        __syncthreads();
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            Four sum = all[(wave * 4 + i) * 64 + lane];
+            #pragma unroll
+            for (int w = 1; w < 4; w++) sum += all[((w * 4 + wave) * 4 + i) * 64 + lane];
+            #pragma unroll
+            for (int r = 0; r < 4; r++) acc[0][i >> 1][0][i & 1][r] = sum[r];
+        }
+    }
+
     // f(row, column, value) for every run of RUN consecutive rows of a column that the lane holds, value(r) its numbers; rows and columns
     // count from the tile's corner
     static constexpr int RUN = AK_ ? 8 : 4;
     template <typename F>
     __device__ __forceinline__ void each(F &&f)
     {
-        int const lane = thread_now() & 63, wave = wave_number(), j = lane & 31, q = lane >> 5;
+        int const lane = thread_now() & 63, wave = wave_number() % (SHARE / 64), part = WAVES_K > 1 ? wave_number() : 0, j = lane & 31, q = lane >> 5;
         int const m0 = wave % WAVES_M * (BM / WAVES_M), n0 = wave / WAVES_M * (BN / WAVES_N);
         #pragma unroll
         for (int x = 0; x < MB; x++)
@@ -375,11 +429,11 @@ struct ProductTile {
                 #pragma unroll
                 for (int u = 0; u < 2; u++)
                     #pragma unroll
-                    for (int g = 0; g < 4; g++)
+                    for (int g = 0; g < (WAVES_K > 1 ? 1 : 4); g++)
                         #pragma unroll
                         for (int t = 0; t < 8 / RUN; t++) {
                             auto const v = [&](int r) { return acc[x][AK_ ? r >> 2 : t][y][u][4 * g + (r & 3)]; };
-                            f(m0 + 64 * x + OA::row(8 * g + 4 * q, t), n0 + 64 * y + OB::row(j, u), v);
+                            f(m0 + 64 * x + OA::row(8 * (g + part) + 4 * q, t), n0 + 64 * y + OB::row(j, u), v);
                         }
     }
 };

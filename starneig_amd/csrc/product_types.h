@@ -49,6 +49,23 @@ struct Span { int group, begin, end; };
 // Offsets come from the device (a router's prefix sums) and are not trusted: each is clamped to [0, n] and to its
 // predecessors' maximum, so that the groups are disjoint and inside the matrix whatever the array holds.
 //
+// Prefix sum / prefix maximum of non-negative numbers over the lanes, and the number of the lane before (lane 0: `first`), by the
+// cross-lane operands of vector instructions (a shuffle through LDS takes ten times as long, and six of them wait for each other).
+template <int CTRL, int ROWS> __device__ __forceinline__ int from_lane(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int prefix_sum(int v)
+{
+    v += from_lane<0x111, 0xf>(v); v += from_lane<0x112, 0xf>(v); v += from_lane<0x114, 0xf>(v); v += from_lane<0x118, 0xf>(v);
+    v += from_lane<0x142, 0xa>(v); v += from_lane<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ int prefix_max(int v)
+{
+    v = max(v, from_lane<0x111, 0xf>(v)); v = max(v, from_lane<0x112, 0xf>(v)); v = max(v, from_lane<0x114, 0xf>(v)); v = max(v, from_lane<0x118, 0xf>(v));
+    v = max(v, from_lane<0x142, 0xa>(v)); v = max(v, from_lane<0x143, 0xc>(v));
+    return v;
+}
+__device__ __forceinline__ int lane_before(int v, int first) { return __builtin_amdgcn_update_dpp(first, v, 0x138, 0xf, 0xf, false); }
+
 // The groups cut into pieces of at most `width` columns, in the groups' order.  Every wave walks by itself, 64 groups at a time: a prefix
 // maximum for the offsets and a prefix sum for the pieces, no shared memory and no barrier; up to 64 groups
 // stay in the lanes, so that a further piece is found without another walk.
@@ -72,14 +89,9 @@ struct Pieces {
         int const lane = threadIdx.x & 63, g = g0 + lane;
         end = g < groups ? offset(g + 1) : 0;
         end = max(end, carry);
-        #pragma unroll
-        for (int d = 1; d < 64; d *= 2) { int const o = __shfl_up(end, d); if (lane >= d) end = max(end, o); }
-        begin = __shfl_up(end, 1);
-        if (lane == 0) begin = carry;
-        int const count = (end - begin + width - 1) / width;
-        int sum = count;
-        #pragma unroll
-        for (int d = 1; d < 64; d *= 2) { int const o = __shfl_up(sum, d); if (lane >= d) sum += o; }
+        end = prefix_max(end);
+        begin = lane_before(end, carry);
+        int const count = (unsigned)(end - begin + width - 1) / (unsigned)width, sum = prefix_sum(count);
         first = before + sum - count;
         before += __builtin_amdgcn_readlane(sum, 63);
         carry = __builtin_amdgcn_readlane(end, 63);
@@ -110,9 +122,7 @@ __device__ __forceinline__ Span whole_group(int const *__restrict__ offsets, int
     int top = 0;
     for (int g0 = 0; g0 <= group; g0 += 64)
         if (g0 + lane <= group) top = max(top, min(max(offsets[g0 + lane], 0), n));
-    #pragma unroll
-    for (int d = 32; d > 0; d /= 2) top = max(top, __shfl_xor(top, d));
-    top = __builtin_amdgcn_readfirstlane(top);
+    top = __builtin_amdgcn_readlane(prefix_max(top), 63);
     int const end = __builtin_amdgcn_readfirstlane(max(min(max(offsets[group + 1], 0), n), top));
     return Span{group, top, end};
 }
@@ -129,10 +139,8 @@ struct Longest {
         int const lane = threadIdx.x & 63;
         int const before = __builtin_amdgcn_readfirstlane(min(max(offsets[0], 0), n));
         end = max(lane < groups ? min(max(offsets[lane + 1], 0), n) : 0, before);
-        #pragma unroll
-        for (int d = 1; d < 64; d *= 2) { int const o = __shfl_up(end, d); if (lane >= d) end = max(end, o); }
-        begin = __shfl_up(end, 1);
-        if (lane == 0) begin = before;
+        end = prefix_max(end);
+        begin = lane_before(end, before);
         int const length = end - begin;
         rank = lane < groups ? 0 : 64;
         for (int g = 0; g < groups; g++) {

@@ -4,6 +4,7 @@
 #include "dgemm_tile.h"
 #include "products.h"
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace sn {
@@ -80,17 +81,17 @@ void grouped_outer_kernel(int groups, int m, int n, int k, int slices, int const
     });
 }
 
-template <typename D>
+template <typename S, typename D>
 __global__ __launch_bounds__(256)
-void grouped_outer_sum_kernel(int groups, int m, int n, int slices, float const *__restrict__ planes, float beta, D *__restrict__ out, long ldd, long strideD)
+void grouped_outer_sum_kernel(int groups, int m, int n, int slices, S const *__restrict__ planes, S beta, D *__restrict__ out, long ldd, long strideD)
 {
     long const all = (long)groups * n * m;
     for (long e = blockIdx.x * 256L + threadIdx.x; e < all; e += gridDim.x * 256L) {
-        float sum = planes[e];
+        S sum = planes[e];
         for (int s = 1; s < slices; s++) sum += planes[s * all + e];
         long const column = e / m;
         D *const to = out + column / n * strideD + column % n * ldd + e % m;
-        *to = (D)(beta == 0.f ? sum : sum + beta * (float)*to);
+        *to = (D)(beta == 0 ? sum : sum + beta * (S)*to);
     }
 }
 
@@ -268,53 +269,60 @@ void grouped_gemm_few_kernel(int groups, int m, int n, int k, int const *__restr
         [&](int r, int c, float sum) { C[(s.begin + c) * ldc + r0 + r] = (T)sum; });
 }
 
-static __device__ __forceinline__ Span piece_of(int const *offsets, int groups, int n, int width, int piece)
-{
-    Pieces pieces(offsets, groups, n, width);
-    return piece < pieces.total ? pieces.at(piece) : Span{-1, 0, 0};
-}
-
-// fp64: the tile of the library's own dgemm, one piece of a group a workgroup
+// fp64: the tile of the library's own dgemm, one piece of a group a workgroup; the tile rows of a piece side by side, so that its columns
+// come from memory once (24 matrices 312 x 312, 40000 columns: 182 us, 43 TFLOP/s; 20000 columns, 8 matrices 1024 x 1024: 757 us, 55 TFLOP/s)
 template <bool TA>
 __global__ __launch_bounds__(256, 2)
 void grouped_dgemm_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, double const *__restrict__ A, int lda, long strideA,
     double const *__restrict__ B, int ldb, double *__restrict__ C, int ldc)
 {
-    Span const s = piece_of(offsets, groups, n, 64, blockIdx.x);
-    if (s.group < 0) return;
+    Pieces pieces(offsets, groups, n, 64);
+    int const rows = (m + 63) / 64, t = tile_of_workgroup(rows * pieces.total, 0);
+    if (t < 0) return;
+    int const row = (unsigned)t % (unsigned)rows;
+    Span const s = pieces.at((unsigned)t / (unsigned)rows);
     if (k == 0) {           // (the tile reads its operands' last inner term: there must be one)
         for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-            int const r = blockIdx.y * 64 + e % 64, c = s.begin + e / 64;
+            int const r = row * 64 + e % 64, c = s.begin + e / 64;
             if (r < m && c < s.end) C[(size_t)c * ldc + r] = 0.0;
         }
         return;
     }
     gemm_tile<64, 64, 16, TA, false, 16>(m, s.end - s.begin, k, 1.0, A + s.group * strideA, lda, B + (size_t)s.begin * ldb, ldb,
-        0.0, C + (size_t)s.begin * ldc, ldc, blockIdx.y, 0);
+        0.0, C + (size_t)s.begin * ldc, ldc, row, 0);
 }
 
+// (cut into slices of the columns like the others: see grouped_outer_kernel)
 __global__ __launch_bounds__(256, 2)
-void grouped_douter_kernel(int m, int n, int k, int const *__restrict__ offsets, double const *__restrict__ X, int ldx,
+void grouped_douter_kernel(int groups, int m, int n, int k, int slices, int const *__restrict__ offsets, double const *__restrict__ X, int ldx,
     double const *__restrict__ Y, int ldy, double beta, double *__restrict__ D, int ldd, long strideD)
 {
-    Span const s = whole_group(offsets, k, blockIdx.z);
-    double *const to = D + s.group * strideD;
-    if (s.begin == s.end) {
+    int const rows = (m + 63) / 64, cols = (n + 63) / 64, each = rows * cols, t = tile_of_workgroup(groups * slices * each, 0);
+    if (t < 0) return;
+    int const in = (unsigned)t % (unsigned)(each * slices), slice = (unsigned)in / (unsigned)each, tile = in - slice * each;
+    int const row = (unsigned)tile % (unsigned)rows, col = (unsigned)tile / (unsigned)rows;
+    Span const s = whole_group(offsets, k, (unsigned)t / (unsigned)(each * slices));
+    int const length = s.end - s.begin, part = slices == 1 ? length : ((length + slices - 1) / slices + 15) / 16 * 16;
+    int const begin = s.begin + (int)min((long)slice * part, (long)length), end = min(begin + part, s.end);
+    double *const to = D + ((long)slice * groups + s.group) * strideD;
+    if (begin == end) {
         for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-            int const r = blockIdx.x * 64 + e % 64, c = blockIdx.y * 64 + e / 64;
+            int const r = row * 64 + e % 64, c = col * 64 + e / 64;
             if (r < m && c < n) { double *const p = to + (size_t)c * ldd + r; *p = beta == 0.0 ? 0.0 : beta * *p; }
         }
         return;
     }
-    gemm_tile<64, 64, 16, false, true, 16>(m, n, s.end - s.begin, 1.0, X + (size_t)s.begin * ldx, ldx, Y + (size_t)s.begin * ldy, ldy,
-        beta, to, ldd, blockIdx.x, blockIdx.y);
+    gemm_tile<64, 64, 16, false, true, 16>(m, n, end - begin, 1.0, X + (size_t)begin * ldx, ldx, Y + (size_t)begin * ldy, ldy,
+        beta, to, ldd, row, col);
 }
 
 template <bool TA>
 static hipError_t dgemm_launch(hipStream_t s, int groups, int m, int n, int k, int const *offsets, double const *A, int lda, long strideA,
     double const *B, int ldb, double *C, int ldc)
 {
-    return launch_kernel(grouped_dgemm_kernel<TA>, dim3((unsigned)most_pieces(groups, n, 64), (m + 63) / 64), 256, s,
+    long const tiles = most_pieces(groups, n, 64) * ((m + 63) / 64);
+    if (tiles >= 1L << 31) return hipErrorInvalidConfiguration;
+    return launch_kernel(grouped_dgemm_kernel<TA>, dim3((unsigned)roundup(tiles, 8)), 256, s,
         GemmCfg<64, 64, 16, TA, false>::LDS_BYTES, groups, m, n, k, offsets, A, lda, strideA, B, ldb, C, ldc);
 }
 
@@ -328,10 +336,41 @@ static bool direct(void const *p, long ld, long stride, int contiguous, int size
 // Workgroups for so many equal tiles: no more than the chip holds at once, each with a run of tiles, so that the loads of the next tile
 // begin while the last one's products end.
 template <typename P>
-static unsigned resident(long tiles) { return (unsigned)std::min<long>(roundup(tiles, 8), 256 * (163840 / P::LDS_BYTES)); }
+static unsigned resident(long tiles)
+{
+    return (unsigned)(P::WAVES_K > 1 ? roundup(tiles, 8) : std::min<long>(roundup(tiles, 8), 256 * (163840 / P::LDS_BYTES)));
+}
 
-// Few columns a group on average, and too few 128 x 128 tiles to fill the chip (which read the matrix as fast where there are enough).
-static bool few_columns(int groups, int m, int n) { return (long)n <= 16L * groups && most_pieces(groups, n, 128) * ((m + 127) / 128) < 256; }
+// What a launch takes, in us, fitted to launches of 64 ... 65536 columns, 1 ... 32 groups, 64 ... 4096 rows and 256 ... 8192 inner terms: rounds of the
+// workgroups that the chip holds at once, each of so many k-tiles and what it takes to begin and to store a tile.  A k-tile takes as long as the
+// memory's latency while few workgroups run, as long as the matrix cores need when they fill the chip.
+//   tile  64: four waves cut the inner index, for products of few outputs;   200 columns, 512 x 8192:  26 us (128: 74 us)
+//   tile 128: two workgroups a compute unit;                                2048 columns, 4096 x 4096: 73 us (64: 124 us, 256: 89 us)
+//   tile 256: the fewest reads a product;                                   4096 columns, 4096 x 4096: 120 us (128: 143 us)
+static double tile_time(int tile, bool fast, double workgroups, double ktiles)
+{
+    double const w = std::max(1.0, workgroups), rounds = std::ceil(w / (tile == 128 ? 512 : 256) - 0.01);
+    if (tile == 64) return rounds * ((fast ? 0.66 : 1.1) * std::ceil(ktiles / 4) + (fast ? 4.9 : 8.6));
+    if (tile == 128) return w <= 256 ? (fast ? 0.62 : 0.9) * ktiles + 6 : rounds * ((fast ? 1.05 : 1.3) * ktiles + 6);
+    return rounds * ((1.1 + 0.65 * std::min(1.0, w / 256)) * ktiles + 8);
+}
+// The tile of a product.  The host does not know the groups' lengths: it counts the pieces that exponentially distributed ones of this mean have.
+static int product_tile(bool fast, int groups, int m, int n, int ktiles)
+{
+    int best = 64;
+    double least = 0;
+    for (int tile : {64, 128, 256}) {
+        if (tile == 256 && !fast) continue;
+        double const some = std::min(groups, n), pieces = groups == 1 ? (n + tile - 1) / tile : some / (1 - std::exp(-tile * some / n));
+        // (a tenth more of what exceeds one a group: a last round of hardly any tiles costs as much as a full one)
+        double const time = tile_time(tile, fast, (pieces + 0.1 * (pieces - std::min(pieces, some))) * ((m + tile - 1) / tile), ktiles);
+        if (tile == 64 || time < least) { best = tile; least = time; }
+    }
+    return best;
+}
+// Few columns a group on average, and too few 64 x 64 tiles to fill the chip: 16 columns, 4096 x 4096: 11 us, in tiles of 64 15 us; 256 columns of 32
+// groups, 2048 x 1408: 62 us, in tiles of 128 32 us.
+static bool few_columns(int groups, int m, int n) { return (long)n <= 16L * groups && most_pieces(groups, n, 64) * ((m + 63) / 64) < 256; }
 
 template <typename T, typename P>
 static hipError_t gemm_tiles(hipStream_t s, int groups, int m, int n, int k, int const *offsets, void const *A, int lda, long strideA,
@@ -358,12 +397,11 @@ static hipError_t gemm_launch(hipStream_t s, int groups, int m, int n, int k, in
         return launch_kernel(grouped_gemm_narrow_kernel<T, T>, dim3((unsigned)most_pieces(groups, n, 4), std::min(m, 65535)), 256, s, 0, groups, m, n, k, offsets,
             (T const *)A, TA ? (long)lda : 1L, TA ? 1L : (long)lda, strideA, (float const *)nullptr, 0L, (T const *)B, (long)ldb, (float const *)nullptr, (T *)C, (long)ldc);
     bool const fast = direct(A, lda, strideA, TA ? k : m, sizeof(T)) && direct(B, ldb, 0, k, sizeof(T));
-    // (the large tile where it leaves no compute unit idle)
-    if (most_pieces(groups, n, 256) * ((m + 255) / 256) >= 256)
-    return (fast ? gemm_tiles<T, ProductTile<T, 256, 256, 2, 4, TA, true, DIRECT>> : gemm_tiles<T, ProductTile<T, 128, 128, 2, 2, TA, true, STAGED>>)
-        (s, groups, m, n, k, offsets, A, lda, strideA, B, ldb, C, ldc);
-    return (fast ? gemm_tiles<T, ProductTile<T, 128, 128, 2, 2, TA, true, DIRECT>> : gemm_tiles<T, ProductTile<T, 128, 128, 2, 2, TA, true, STAGED>>)
-        (s, groups, m, n, k, offsets, A, lda, strideA, B, ldb, C, ldc);
+    int const tile = product_tile(fast, groups, m, n, (k + 63) / 64);
+    auto const launch = fast ? tile == 256 ? gemm_tiles<T, ProductTile<T, 256, 256, 2, 4, TA, true, DIRECT>> : tile == 128 ? gemm_tiles<T, ProductTile<T, 128, 128, 2, 2, TA, true, DIRECT>>
+            : gemm_tiles<T, ProductTile<T, 64, 64, 1, 1, TA, true, DIRECT, 4>>
+        : tile == 128 ? gemm_tiles<T, ProductTile<T, 128, 128, 2, 2, TA, true, STAGED>> : gemm_tiles<T, ProductTile<T, 64, 64, 1, 1, TA, true, STAGED, 4>>;
+    return launch(s, groups, m, n, k, offsets, A, lda, strideA, B, ldb, C, ldc);
 }
 
 hipError_t grouped_gemm(hipStream_t s, ProductType type, bool transA, int groups, int m, int n, int k, int const *offsets,
@@ -375,15 +413,12 @@ hipError_t grouped_gemm(hipStream_t s, ProductType type, bool transA, int groups
     return launch(s, groups, m, n, k, offsets, (double const *)A, lda, strideA, (double const *)B, ldb, (double *)C, ldc);
 }
 
-// What a launch takes, in us: rounds of the workgroups that the chip holds at once, each of so many k-tiles (and what six of them take to begin and
-// to store a tile), plus, cut into slices, writing and reading the planes and a second launch.
+// A weight gradient's tile and the slices that its columns are cut into: with slices there is a plane to write and read for each, and a second launch.
 struct Cut { int tile, slices; };
-static double outer_time(Cut c, long groups, long m, long n, long k)
+static double outer_time(Cut c, bool fast, long groups, long m, long n, long k)
 {
     long const items = groups * ((m + c.tile - 1) / c.tile) * ((n + c.tile - 1) / c.tile) * c.slices;
-    long const held = c.tile == 256 ? 256 : 512, rounds = (items + held - 1) / held;
-    double const tiles = (double)k / groups / c.slices / 64;
-    return rounds * (tiles + 6) * (c.tile == 256 ? 1.8 : 1.2) + (c.slices > 1 ? 3 + c.slices * (double)groups * m * n * 8 / 4e6 : 0);
+    return tile_time(c.tile, fast, items, (double)k / groups / c.slices / 64) + (c.slices > 1 ? 3 + c.slices * (double)groups * m * n * 8 / 4e6 : 0);
 }
 static Cut outer_cut(bool fast, long groups, long m, long n, long k)
 {
@@ -392,7 +427,7 @@ static Cut outer_cut(bool fast, long groups, long m, long n, long k)
         for (int slices : {1, 2, 4, 8, 16, 32, 64}) {
             Cut const c = {tile, slices};
             if ((tile == 256 && !fast) || (slices > 1 && k / groups / slices < 64)) continue;
-            if (outer_time(c, groups, m, n, k) < outer_time(best, groups, m, n, k)) best = c;
+            if (outer_time(c, fast, groups, m, n, k) < outer_time(best, fast, groups, m, n, k)) best = c;
         }
     return best;
 }
@@ -427,13 +462,21 @@ static hipError_t outer_launch(hipStream_t s, int groups, int m, int n, int k, i
     if (c.slices == 1) return go((D *)out, ldd, strideD, beta);
     hipError_t const e = go((float *)work, m, (long)m * n, 0.0);
     if (e != hipSuccess) return e;
-    return launch_kernel(grouped_outer_sum_kernel<D>, dim3((unsigned)std::min(((long)groups * m * n + 255) / 256, 4096L)), 256, s, 0,
+    return launch_kernel(grouped_outer_sum_kernel<float, D>, dim3((unsigned)std::min(((long)groups * m * n + 255) / 256, 4096L)), 256, s, 0,
         groups, m, n, c.slices, (float const *)work, (float)beta, (D *)out, (long)ldd, strideD);
+}
+
+// fp64: as many slices as fill the chip's three workgroups a compute unit, of 256 columns at least
+static int douter_slices(long groups, long m, long n, long k)
+{
+    long const tiles = groups * ((m + 63) / 64) * ((n + 63) / 64);
+    return (int)std::max(1L, std::min({768 / tiles, k / groups / 256, 64L}));
 }
 
 long grouped_outer_work_size(ProductType type, int groups, int m, int n, int k)
 {
-    if (type == PRODUCT_F64 || m < 8 || n < 8) return 0;
+    if (type == PRODUCT_F64) { int const slices = douter_slices(groups, m, n, k); return slices > 1 ? (long)slices * groups * m * n * 8 : 0; }
+    if (m < 8 || n < 8) return 0;
     // (whichever way the operands are aligned)
     int const slices = std::max(outer_cut(true, groups, m, n, k).slices, outer_cut(false, groups, m, n, k).slices);
     return slices > 1 ? (long)slices * groups * m * n * 4 : 0;
@@ -442,9 +485,17 @@ long grouped_outer_work_size(ProductType type, int groups, int m, int n, int k)
 hipError_t grouped_outer(hipStream_t s, ProductType type, ProductType typeD, int groups, int m, int n, int k, int const *offsets,
     void const *X, int ldx, void const *Y, int ldy, double beta, void *D, int ldd, long strideD, void *work, long work_size)
 {
-    if (type == PRODUCT_F64)
-        return launch_kernel(grouped_douter_kernel, dim3((m + 63) / 64, (n + 63) / 64, groups), 256, s, GemmCfg<64, 64, 16, false, true>::LDS_BYTES,
-            m, n, k, offsets, (double const *)X, ldx, (double const *)Y, ldy, beta, (double *)D, ldd, strideD);
+    if (type == PRODUCT_F64) {
+        int const slices = work != nullptr && work_size >= grouped_outer_work_size(type, groups, m, n, k) ? douter_slices(groups, m, n, k) : 1;
+        long const tiles = (long)groups * slices * ((m + 63) / 64) * ((n + 63) / 64);
+        if (tiles >= 1L << 31) return hipErrorInvalidConfiguration;
+        hipError_t const e = launch_kernel(grouped_douter_kernel, dim3((unsigned)roundup(tiles, 8)), 256, s, GemmCfg<64, 64, 16, false, true>::LDS_BYTES,
+            groups, m, n, k, slices, offsets, (double const *)X, ldx, (double const *)Y, ldy, slices > 1 ? 0.0 : beta,
+            slices > 1 ? (double *)work : (double *)D, slices > 1 ? m : ldd, slices > 1 ? (long)m * n : strideD);
+        if (e != hipSuccess || slices == 1) return e;
+        return launch_kernel(grouped_outer_sum_kernel<double, double>, dim3((unsigned)std::min(((long)groups * m * n + 255) / 256, 4096L)), 256, s, 0,
+            groups, m, n, slices, (double const *)work, beta, (double *)D, (long)ldd, strideD);
+    }
     bool const wide = typeD == PRODUCT_F32;
     auto const launch = type == PRODUCT_BF16 ? (wide ? outer_launch<__bf16, float> : outer_launch<__bf16, __bf16>)
                                              : (wide ? outer_launch<_Float16, float> : outer_launch<_Float16, _Float16>);
@@ -495,12 +546,11 @@ static hipError_t gemm_i8_launch(hipStream_t s, int groups, int m, int n, int k,
             A, (long)lda, 1L, strideA, scaleA, strideS, B, (long)ldb, scaleB, (D *)C, (long)ldc);
     bool const fast = direct(A, lda, strideA, k, 1) && direct(B, ldb, 0, k, 1);
     typedef signed char T;
-    // (the large tile where it leaves no compute unit idle)
-    if (most_pieces(groups, n, 256) * ((m + 255) / 256) >= 256)
-    return (fast ? gemm_i8_tiles<D, ProductTile<T, 256, 256, 2, 4, true, true, DIRECT>> : gemm_i8_tiles<D, ProductTile<T, 128, 128, 2, 2, true, true, STAGED>>)
-        (s, groups, m, n, k, offsets, A, lda, strideA, scaleA, strideS, B, ldb, scaleB, C, ldc);
-    return (fast ? gemm_i8_tiles<D, ProductTile<T, 128, 128, 2, 2, true, true, DIRECT>> : gemm_i8_tiles<D, ProductTile<T, 128, 128, 2, 2, true, true, STAGED>>)
-        (s, groups, m, n, k, offsets, A, lda, strideA, scaleA, strideS, B, ldb, scaleB, C, ldc);
+    int const tile = product_tile(fast, groups, m, n, (k + 127) / 128);
+    auto const launch = fast ? tile == 256 ? gemm_i8_tiles<D, ProductTile<T, 256, 256, 2, 4, true, true, DIRECT>> : tile == 128 ? gemm_i8_tiles<D, ProductTile<T, 128, 128, 2, 2, true, true, DIRECT>>
+            : gemm_i8_tiles<D, ProductTile<T, 64, 64, 1, 1, true, true, DIRECT, 4>>
+        : tile == 128 ? gemm_i8_tiles<D, ProductTile<T, 128, 128, 2, 2, true, true, STAGED>> : gemm_i8_tiles<D, ProductTile<T, 64, 64, 1, 1, true, true, STAGED, 4>>;
+    return launch(s, groups, m, n, k, offsets, A, lda, strideA, scaleA, strideS, B, ldb, scaleB, C, ldc);
 }
 
 hipError_t gemm_i8(hipStream_t s, ProductType typeC, int groups, int m, int n, int k, int const *offsets, signed char const *A, int lda, long strideA,

@@ -76,7 +76,8 @@ def test_work_size():
     size = S.lib.load().starneig_amd_grouped_outer_work_size
     assert size(S.AMD_BF16, 1, 512, 384, 20000) % (512 * 384 * 4) == 0 and size(S.AMD_BF16, 1, 512, 384, 20000) > 0      # few outputs, a long sum
     assert size(S.AMD_F16, 16, 4096, 2048, 32768) == 0              # outputs enough
-    assert size(S.AMD_F64, 1, 512, 384, 20000) == 0
+    assert size(S.AMD_F64, 1, 512, 384, 20000) % (512 * 384 * 8) == 0 and size(S.AMD_F64, 1, 512, 384, 20000) > 0
+    assert size(S.AMD_F64, 24, 312, 312, 40000) == 0
     for refused in [(S.AMD_F32, 1, 512, 384, 20000), (9, 1, 512, 384, 20000), (S.AMD_BF16, 0, 512, 384, 20000), (S.AMD_BF16, 65536, 512, 384, 20000),
                     (S.AMD_BF16, 1, 0, 384, 20000), (S.AMD_BF16, 1, 512, -1, 20000), (S.AMD_BF16, 1, 512, 384, 0)]:
         assert size(*refused) == 0
