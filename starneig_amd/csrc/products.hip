@@ -12,6 +12,40 @@ namespace sn {
 // a tile's place in the matrices
 struct Place { Span s; bool there; };
 
+// Where a tile goes: high x wide numbers from `to` on exist.  put: WHOLE, without a look at these.
+template <typename D>
+struct Columns {
+    static constexpr bool FREE = true;          // worth code of its own without the tests
+    D *to;
+    long ld;
+    int high, wide;
+    __device__ __forceinline__ int rows() const { return high; }
+    __device__ __forceinline__ int cols() const { return wide; }
+    template <bool WHOLE, int N> __device__ __forceinline__ void put(int r, int c, D const (&v)[N]) const
+    {
+        if (WHOLE || c < wide) store_run<WHOLE>(to + c * ld + r, high - r, v);
+    }
+};
+// The same for sums in fp32 that are added to beta times what is there.
+template <typename D>
+struct Added : Columns<D> {
+    static constexpr bool FREE = false;
+    float beta;
+    template <bool WHOLE> __device__ __forceinline__ void put(int r, int c, float const (&v)[4]) const
+    {
+        if (!WHOLE && c >= this->wide) return;
+        D *const at = this->to + c * this->ld + r;
+        D sum[4];
+        if (WHOLE || r + 4 <= this->high) __builtin_memcpy(sum, at, sizeof sum);
+        else
+            #pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] = r + e < this->high ? at[e] : (D)0.f;
+        #pragma unroll
+        for (int e = 0; e < 4; e++) sum[e] = (D)(v[e] + beta * (float)sum[e]);
+        store_run<WHOLE>(at, this->high - r, sum);
+    }
+};
+
 template <typename T, typename P>
 __global__ __launch_bounds__(P::THREADS, P::PER_SIMD)
 void grouped_gemm_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, T const *__restrict__ A, long lda, long strideA,
@@ -31,9 +65,8 @@ void grouped_gemm_kernel(int groups, int m, int n, int k, int const *__restrict_
         p = Plan<T>{A + s.group * strideA + r0 * (P::A_K ? lda : 1L), B + s.begin * ldb, lda, ldb, m - r0, s.end - s.begin, k, r0, 0};
         return Place{s, true};
     }, [&](Plan<T> const &p, Place const &at) {
-        tile.each([&](int r, int c, auto &&value) {
-            if (at.s.begin + c < at.s.end) store_run<P::RUN>(C + (at.s.begin + c) * ldc + p.r0 + r, m - p.r0 - r, value);
-        });
+        tile.template store<T>(lds, [&](int x, int t, int y, int u, int r) { return (T)tile.acc[x][t][y][u][r]; },
+            Columns<T>{C + at.s.begin * ldc + p.r0, ldc, p.rows, p.cols});
     });
 }
 
@@ -64,20 +97,9 @@ void grouped_outer_kernel(int groups, int m, int n, int k, int slices, int const
         p = Plan<T>{X + begin * ldx + r0, Y + begin * ldy + c0, ldx, ldy, m - r0, n - c0, end - begin, r0, c0};
         return Place{s.group, slice, true};
     }, [&](Plan<T> const &p, Place const &at) {
-        D *const to = out + ((long)at.slice * groups + at.group) * strideD;
-        tile.each([&](int r, int c, auto &&value) {
-            if (p.c0 + c >= n) return;
-            D *const d = to + (p.c0 + c) * ldd + p.r0 + r;
-            int const left = m - p.r0 - r;
-            if (beta != 0.f) {
-                // (all old values are asked for before any is overwritten)
-                float old[P::RUN];
-                #pragma unroll
-                for (int e = 0; e < P::RUN; e++) old[e] = e < left ? (float)d[e] : 0.f;
-                store_run<P::RUN>(d, left, [&](int e) { return value(e) + beta * old[e]; });
-            } else
-                store_run<P::RUN>(d, left, value);
-        });
+        Columns<D> const to{out + ((long)at.slice * groups + at.group) * strideD + p.c0 * ldd + p.r0, ldd, p.rows, p.cols};
+        if (beta == 0.f) tile.template store<D>(lds, [&](int x, int t, int y, int u, int r) { return (D)tile.acc[x][t][y][u][r]; }, to);
+        else tile.template store<float>(lds, [&](int x, int t, int y, int u, int r) { return tile.acc[x][t][y][u][r]; }, Added<D>{to, beta});
     });
 }
 
@@ -104,6 +126,20 @@ __device__ __forceinline__ float scaled(int sum, float row, float col)
     return v;
 }
 
+template <typename D>
+struct Scaled : Columns<D> {
+    float const *row, *col;
+    template <bool WHOLE> __device__ __forceinline__ void put(int r, int c, int const (&v)[4]) const
+    {
+        if (!WHOLE && c >= this->wide) return;
+        float const scale = col[c];
+        D d[4];
+        #pragma unroll
+        for (int e = 0; e < 4; e++) d[e] = (D)scaled(v[e], row[WHOLE ? r + e : min(r + e, this->high - 1)], scale);
+        store_run<WHOLE>(this->to + c * this->ld + r, this->high - r, d);
+    }
+};
+
 template <typename D, typename P>
 __global__ __launch_bounds__(P::THREADS, P::PER_SIMD)
 void gemm_i8_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, signed char const *__restrict__ A, long lda, long strideA,
@@ -124,13 +160,8 @@ void gemm_i8_kernel(int groups, int m, int n, int k, int const *__restrict__ off
         p = Plan<T>{A + s.group * strideA + r0 * lda, B + s.begin * ldb, lda, ldb, m - r0, s.end - s.begin, k, r0, 0};
         return Place{s, true};
     }, [&](Plan<T> const &p, Place const &at) {
-        float const *const sa = scaleA + at.s.group * strideS + p.r0;
-        tile.each([&](int r, int c, auto &&value) {
-            if (at.s.begin + c >= at.s.end) return;
-            float const col = scaleB[at.s.begin + c];
-            int const left = m - p.r0 - r;
-            store_run<P::RUN>(C + (at.s.begin + c) * ldc + p.r0 + r, left, [&](int e) { return scaled(value(e), e < left ? sa[r + e] : 0.f, col); });
-        });
+        tile.template store<int>(lds, [&](int x, int t, int y, int u, int r) { return tile.acc[x][t][y][u][r]; },
+            Scaled<D>{{C + at.s.begin * ldc + p.r0, ldc, p.rows, p.cols}, scaleA + at.s.group * strideS + p.r0, scaleB + at.s.begin});
     });
 }
 
@@ -361,9 +392,10 @@ static int product_tile(bool fast, int groups, int m, int n, int ktiles)
     double least = 0;
     for (int tile : {64, 128, 256}) {
         if (tile == 256 && !fast) continue;
-        double const some = std::min(groups, n), pieces = groups == 1 ? (n + tile - 1) / tile : some / (1 - std::exp(-tile * some / n));
-        // (a tenth more of what exceeds one a group: a last round of hardly any tiles costs as much as a full one)
-        double const time = tile_time(tile, fast, (pieces + 0.1 * (pieces - std::min(pieces, some))) * ((m + tile - 1) / tile), ktiles);
+        // (and a tenth more of what exceeds one a group: a last round of hardly any tiles costs as much as a full one)
+        double const some = std::min(groups, n), expected = some / (1 - std::exp(-tile * some / n));
+        double const pieces = groups == 1 ? (n + tile - 1) / tile : expected + 0.1 * (expected - some);
+        double const time = tile_time(tile, fast, pieces * ((m + tile - 1) / tile), ktiles);
         if (tile == 64 || time < least) { best = tile; least = time; }
     }
     return best;
@@ -423,7 +455,7 @@ static double outer_time(Cut c, bool fast, long groups, long m, long n, long k)
 static Cut outer_cut(bool fast, long groups, long m, long n, long k)
 {
     Cut best = {128, 1};
-    for (int tile : {256, 128})
+    for (int tile : {256, 128, 64})
         for (int slices : {1, 2, 4, 8, 16, 32, 64}) {
             Cut const c = {tile, slices};
             if ((tile == 256 && !fast) || (slices > 1 && k / groups / slices < 64)) continue;
@@ -456,7 +488,8 @@ static hipError_t outer_launch(hipStream_t s, int groups, int m, int n, int k, i
     auto const go = [&](auto *to, int ld, long stride, double b) {
         typedef std::remove_pointer_t<decltype(to)> O;
         auto const launch = c.tile == 256 ? outer_tiles<T, O, ProductTile<T, 256, 256, 2, 4, false, false, DIRECT>>
-            : fast ? outer_tiles<T, O, ProductTile<T, 128, 128, 2, 2, false, false, DIRECT>> : outer_tiles<T, O, ProductTile<T, 128, 128, 2, 2, false, false, STAGED>>;
+            : c.tile == 128 ? fast ? outer_tiles<T, O, ProductTile<T, 128, 128, 2, 2, false, false, DIRECT>> : outer_tiles<T, O, ProductTile<T, 128, 128, 2, 2, false, false, STAGED>>
+            : fast ? outer_tiles<T, O, ProductTile<T, 64, 64, 1, 1, false, false, DIRECT, 4>> : outer_tiles<T, O, ProductTile<T, 64, 64, 1, 1, false, false, STAGED, 4>>;
         return launch(s, c.slices, groups, m, n, k, offsets, X, ldx, Y, ldy, b, to, ld, stride);
     };
     if (c.slices == 1) return go((D *)out, ldd, strideD, beta);
