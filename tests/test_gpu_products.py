@@ -481,6 +481,105 @@ def test_experts_in_8_bits(node):
         assert bool(((h[a:b].double() - ref).abs() <= half * 1.01 + ref.abs() * 2 ** -8).all())
 
 
+@pytest.mark.parametrize("type_", ["bf16", "f64"])
+def test_gradients_without_scratch_memory(node, type_):
+    """The C call with no scratch memory, with too little and with enough: all within the bound, equal calls equal bits."""
+    import torch
+    gen, k, m, n = generator(51), 20000, 200, 136
+    X = torch.randn(k, m, generator=gen, device="cuda", dtype=torch.float64).to(kind(type_))
+    Y = torch.randn(k, n, generator=gen, device="cuda", dtype=torch.float64).to(kind(type_))
+    off = offsets_of([k - 70], 40)
+    lib, code = node.lib.load(), {"bf16": node.AMD_BF16, "f64": node.AMD_F64}[type_]
+    size = lib.starneig_amd_grouped_outer_work_size(code, 1, m, n, k)
+    assert size > 0
+    work = torch.full((size + 16,), 171, dtype=torch.uint8, device="cuda")
+    x, y = X[40:k - 30].double(), Y[40:k - 30].double()
+    ref, mag = y.T @ x, y.T.abs() @ x.abs()
+    bound = product_bound(k, mag, ref, kind(type_))
+    stream = torch.cuda.current_stream().cuda_stream
+    for given in (0, 16, size - 16, size):
+        got = []
+        for _ in range(2):
+            D = torch.full((1, n, m), float("nan"), dtype=kind(type_), device="cuda")
+            assert lib.starneig_amd_grouped_outer_device(code, code, 1, m, n, k, off.data_ptr(), X.data_ptr(), m, Y.data_ptr(), n, 0.0,
+                                                         D.data_ptr(), m, m * n, work.data_ptr() if given else None, given, stream) == 0
+            got.append(D)
+        assert torch.equal(got[0], got[1])
+        assert bool(((got[0][0].double() - ref).abs() <= bound).all())
+    assert bool((work[size:] == 171).all())
+
+
+def test_two_gradients_at_once_in_a_graph(node):
+    """Two long sums on two branches of one graph, each with scratch memory of its own: every replay equals the eager results."""
+    import torch
+    gen = generator(52)
+    data = [(torch.randn(16000, 192, generator=gen, device="cuda").bfloat16(), torch.randn(16000, 128, generator=gen, device="cuda").bfloat16(),
+             torch.zeros(1, 128, 192, device="cuda")) for _ in range(2)]
+    off = offsets_of([16000])
+
+    def both():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            assert node.grouped_outer_device(off, *data[1]) == 0
+        assert node.grouped_outer_device(off, *data[0]) == 0
+        torch.cuda.current_stream().wait_stream(side)
+
+    both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        both()
+    for _ in range(4):
+        for x, y, d in data:
+            x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+            d.fill_(-1)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y, d in data:
+            eager = torch.empty_like(d)
+            assert node.grouped_outer_device(off, x, y, eager) == 0
+            assert torch.equal(d, eager)
+
+
+def test_equal_calls_give_equal_bits(node):
+    import torch
+    gen = generator(53)
+    sizes, m, k = [700, 0, 3, 1500], 520, 712
+    A = torch.randn(len(sizes), m, k, generator=gen, device="cuda").half()
+    B = torch.randn(sum(sizes), k, generator=gen, device="cuda").half()
+    off, seen = offsets_of(sizes), []
+    for _ in range(5):
+        C = torch.empty(sum(sizes), m, dtype=torch.float16, device="cuda")
+        D = torch.empty(len(sizes), m, k, device="cuda")
+        assert node.grouped_gemm_device("T", off, A, B, C) == 0
+        assert node.grouped_outer_device(off, B, C, D) == 0
+        seen.append((C, D))
+    assert all(torch.equal(c, seen[0][0]) and torch.equal(d, seen[0][1]) for c, d in seen)
+
+
+def test_infinities_and_nan_stay_in_their_columns(node):
+    """A column that holds an infinity or a NaN spoils its own results and no others, also next to a group's end and in a cut last inner chunk."""
+    import torch
+    gen = generator(54)
+    for k in (72, 203, 640):
+        sizes = [65, 3, 130]
+        n = sum(sizes)
+        A = torch.randn(3, 96, k, generator=gen, device="cuda").bfloat16()
+        B = torch.randn(n, k, generator=gen, device="cuda").bfloat16()
+        clean = torch.empty(n, 96, dtype=torch.bfloat16, device="cuda")
+        assert node.grouped_gemm_device("T", offsets_of(sizes), A, B, clean) == 0
+        bad = [0, 64, 65, 67, n - 1]
+        for i, c in enumerate(bad):
+            B[c, (k - 1) * (i % 2)] = float("nan") if i % 3 else float("inf")
+        C = torch.empty_like(clean)
+        assert node.grouped_gemm_device("T", offsets_of(sizes), A, B, C) == 0
+        fine = torch.ones(n, dtype=torch.bool, device="cuda")
+        fine[bad] = False
+        assert torch.equal(C[fine], clean[fine])
+        assert not bool(C[~fine].isfinite().any())
+
+
 def test_two_streams_at_once(node):
     import torch
     cases = [experts_case(torch.bfloat16, seed=s, tokens=400, groups=8, d=256, hidden=512) for s in (31, 32)]
