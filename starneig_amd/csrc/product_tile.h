@@ -20,8 +20,8 @@ typedef __attribute__((address_space(3))) char lds_char;
 typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// How an operand is brought into LDS: DIRECT = buffer loads that write LDS themselves (16-byte aligned columns, whole chunks), no registers and
-// no LDS instructions; STAGED = through registers, any alignment and any extent.
+// How an operand is brought into LDS: DIRECT = buffer loads that write LDS themselves (columns aligned to 4 bytes), no registers and
+// no LDS instructions; STAGED = through registers, any alignment.
 enum Feed { DIRECT, STAGED };
 
 // A buffer of `bytes` bytes from `p` on: loads from offsets beyond it give zeros.
@@ -67,6 +67,21 @@ struct Operand {
         else   { inner = e / CR; outer = ((e % CR) ^ swizzle_mn(inner)) * EL; }
     }
 
+    // K, a k-tile in LDS of which `left` inner terms exist: zeroes those behind them in the chunk that k cuts (it brought whatever lay there)
+    static __device__ __forceinline__ void trim(lds_char *lds, int left)
+    {
+        i32x4 mask;
+        #pragma unroll
+        for (int w = 0; w < 4; w++) {
+            int const bits = min(max(left % EL * 8 * (int)sizeof(T) - 32 * w, 0), 32);
+            mask[w] = bits == 32 ? -1 : (int)((1u << bits) - 1);
+        }
+        for (int r = thread_now() % THREADS; r < ROWS; r += THREADS) {
+            lds_i32x4 *const at = (lds_i32x4 *)(lds + r * 128 + ((left / EL ^ swizzle_k(r)) << 4));
+            *at = *at & mask;
+        }
+    }
+
     // fragment t of the 64 rows from `row0`, 32 bytes of inner index number `step` of 4
     static __device__ __forceinline__ i32x4 fragment(lds_char const *lds, int row0, int t, int step)
     {
@@ -98,28 +113,30 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
     using O = Operand<T, ROWS, K, THREADS>;
     T const *base;
     long step;                      // MN: numbers between k-tiles
-    int k;
+    int k, ld, outers;
     unsigned at[O::LOADS];          // byte offsets of the thread's chunks; beyond the buffer where there is nothing to read
 
-    __device__ __forceinline__ void set(T const *base_, int outers, int k_, long ld)
+    __device__ __forceinline__ void set(T const *base_, int outers_, int k_, long ld_)
     {
-        base = base_; step = ld * O::KT; k = k_;
+        base = base_; k = k_; ld = (int)ld_; outers = outers_; step = ld_ * O::KT;
         int const thread = thread_now() % THREADS;
         #pragma unroll
         for (int s = 0; s < O::LOADS; s++) {
             int outer, in;
             O::chunk(s * THREADS + thread, outer, in);
             int const far = K ? outer : in, near = K ? in : outer;
-            at[s] = outer < outers ? (unsigned)(far * (int)(ld * sizeof(T)) + near * (int)sizeof(T)) : 0x80000000u;
+            at[s] = outer < outers ? (unsigned)((far * ld + near) * (int)sizeof(T)) : 0x80000000u;
         }
     }
-    // Loads 0 ... LOADS - 1 of k-tile kt to `lds`, after begin(kt); k-tiles are fetched in order.  Offsets from 2^31 on read zeros: positions
-    // past the outer end, and, from the k-tile on that k cuts, the chunks past k.  Behind the last k-tile the buffer is empty.
+    // Loads 0 ... LOADS - 1 of k-tile kt to `lds`, after begin(kt); k-tiles are fetched in order.  Offsets from 2^31 on read zeros: positions past the
+    // outer end, and, in the last k-tile, the chunks past k.  So do the words past the operand's end there, with which a chunk that starts in front of
+    // it may end.  (Words, four bytes: the hardware tests each.)  Behind the last k-tile the buffer is empty.
     i32x4 from;
     __device__ __forceinline__ void begin(int kt)
     {
         int const left = k - kt * O::KT;
-        if (left < O::KT && left > 0) {
+        int bytes = left > 0 ? 0x7fffffff : 0;
+        if (left <= O::KT && left > 0) {
             int const thread = thread_now() % THREADS;
             #pragma unroll
             for (int s = 0; s < O::LOADS; s++) {
@@ -127,8 +144,9 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
                 O::chunk(s * THREADS + thread, outer, inner);
                 if (inner >= left) at[s] = 0x80000000u;
             }
+            bytes = (K ? (min(outers, ROWS) - 1) * ld + left : (left - 1) * ld + min(outers, ROWS + O::EL)) * (int)sizeof(T) + 3 & ~3;
         }
-        from = buffer(K ? base + (long)kt * O::KT : base + kt * step, left > 0 ? 0x7fffffff : 0);
+        from = buffer(K ? base + (long)kt * O::KT : base + kt * step, bytes);
     }
     __device__ __forceinline__ void load(int lds, int s) const { load_to_lds(from, at[s], lds + wave_number() % (THREADS / 64) * 1024 + s * THREADS * 16); }
     __device__ __forceinline__ void fetch(int lds, int kt)
@@ -281,6 +299,16 @@ struct ProductTile {
     __device__ __forceinline__ void set_a(Plan<T> const &p) { a.set(p.A, p.rows, p.k, p.lda); }
     __device__ __forceinline__ void set_b(Plan<T> const &p) { b.set(p.B, p.cols, p.k, p.ldb); }
 
+    // The k-tile whose chunks are cut by k, -1: none
+    static __device__ __forceinline__ int cut_tile(int k) { return (AK_ || BK_) && k % OA::EL != 0 ? k / KT : -1; }
+    __device__ __forceinline__ void trim(lds_char *lds, int place, int k)
+    {
+        if (AK_) OA::trim(lds + place, k % KT);
+        if (BK_) OB::trim(lds + after(place, 1), k % KT);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if constexpr (WAVES_K == 1) asm volatile("s_barrier" ::: "memory");
+    }
+
     // before the first tile
     __device__ __forceinline__ void start(Plan<T> const &p, char *shared)
     {
@@ -290,6 +318,7 @@ struct ProductTile {
             int const lds0 = __builtin_amdgcn_readfirstlane((int)(unsigned long long)lds);
             a.fetch(lds0, 0); b.fetch(lds0 + PLACE, 0); a.fetch(lds0 + 2 * PLACE, 1); b.fetch(lds0 + 3 * PLACE, 1);
             meet<OA::LOADS + OB::LOADS>();
+            if (cut_tile(p.k) == 0) trim(lds, 0, p.k);
             #pragma unroll
             for (int r = 0; r < READS; r++) read(f[0], lds, lds + PLACE, 0, r);
             now = 0;
@@ -310,7 +339,7 @@ struct ProductTile {
                     for (int u = 0; u < 2; u++) acc[x][t][y][u] = Acc{};
         int const tiles = tiles_of(p.k);
         if constexpr (FEED_ == DIRECT) {
-            int const lds0 = __builtin_amdgcn_readfirstlane((int)(unsigned long long)lds);
+            int const lds0 = __builtin_amdgcn_readfirstlane((int)(unsigned long long)lds), cut = cut_tile(p.k);
             for (int kt = 0; kt < tiles; kt++) {
                 int const place = after(now, 2), ahead = kt + 2 < tiles ? kt + 2 : kt + 2 - tiles;
                 if (kt + 2 == tiles) set_a(next);
@@ -318,6 +347,9 @@ struct ProductTile {
                 turn(f[0], f[1], lds + now, lds + after(now, 1), 1, a, lds0 + after(now, 4));
                 // the next k-tile is there, and no wave reads this one's places any more
                 meet<OA::LOADS>();
+                // (kt + 1 == tiles: the next tile's first)
+                if (kt + 1 == cut) trim(lds, place, p.k);
+                if (kt + 1 == tiles && cut_tile(next.k) == 0) trim(lds, place, next.k);
                 if (kt + 2 == tiles) set_b(next);
                 b.begin(ahead);
                 turn(f[1], f[0], lds + place, lds + after(place, 1), 0, b, lds0 + now);

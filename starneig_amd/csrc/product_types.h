@@ -91,16 +91,16 @@ struct Pieces {
         end = max(end, carry);
         end = prefix_max(end);
         begin = lane_before(end, carry);
-        int const count = (unsigned)(end - begin + width - 1) / (unsigned)width, sum = prefix_sum(count);
+        int const count = ((unsigned)(end - begin) + width - 1) / (unsigned)width, sum = prefix_sum(count);
         first = before + sum - count;
         before += __builtin_amdgcn_readlane(sum, 63);
         carry = __builtin_amdgcn_readlane(end, 63);
     }
-    // piece number `piece` < total
+    // Piece number `piece` < total.  (None of its columns where the offsets have changed meanwhile, which they must not.)
     __device__ __forceinline__ Span at(int piece)
     {
         if (groups > 64) start();
-        for (int g0 = 0;; g0 += 64) {
+        for (int g0 = 0; g0 < groups; g0 += 64) {
             if (groups > 64) walk(g0);
             unsigned long long const here = __ballot(piece >= first && (long)(piece - first) * width < end - begin);
             if (here) {
@@ -108,10 +108,11 @@ struct Pieces {
                 Span s;
                 s.group = g0 + l;
                 s.begin = __builtin_amdgcn_readlane(begin, l) + (piece - __builtin_amdgcn_readlane(first, l)) * width;
-                s.end = min(s.begin + width, __builtin_amdgcn_readlane(end, l));
+                s.end = s.begin + min(width, __builtin_amdgcn_readlane(end, l) - s.begin);
                 return s;
             }
         }
+        return Span{0, 0, 0};
     }
 };
 

@@ -357,11 +357,10 @@ static hipError_t dgemm_launch(hipStream_t s, int groups, int m, int n, int k, i
         GemmCfg<64, 64, 16, TA, false>::LDS_BYTES, groups, m, n, k, offsets, A, lda, strideA, B, ldb, C, ldc);
 }
 
-// Whether an operand can be fed directly: 16-byte aligned columns of whole chunks, positions within a tile below 2^31 bytes
-// (256 columns of up to 4 MB).
-static bool direct(void const *p, long ld, long stride, int contiguous, int size)
+// Whether an operand can be fed directly: columns aligned to 4 bytes, positions within a tile below 2^31 bytes (256 columns of up to 4 MB).
+static bool direct(void const *p, long ld, long stride, int size)
 {
-    return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0 && stride * size % 16 == 0 && (long)contiguous * size % 16 == 0 && ld * size <= 1 << 22;
+    return (uintptr_t)p % 4 == 0 && ld * size % 4 == 0 && stride * size % 4 == 0 && ld * size <= 1 << 22;
 }
 
 // Workgroups for so many equal tiles: no more than the chip holds at once, each with a run of tiles, so that the loads of the next tile
@@ -425,10 +424,10 @@ static hipError_t gemm_launch(hipStream_t s, int groups, int m, int n, int k, in
         };
         return go(grouped_gemm_few_kernel<T, 1>, 16);
     }
-    if (k < 8 || (!TA && m < 8))
+    bool const fast = direct(A, lda, strideA, sizeof(T)) && direct(B, ldb, 0, sizeof(T));
+    if (!fast && (k < 8 || (!TA && m < 8)))
         return launch_kernel(grouped_gemm_narrow_kernel<T, T>, dim3((unsigned)most_pieces(groups, n, 4), std::min(m, 65535)), 256, s, 0, groups, m, n, k, offsets,
             (T const *)A, TA ? (long)lda : 1L, TA ? 1L : (long)lda, strideA, (float const *)nullptr, 0L, (T const *)B, (long)ldb, (float const *)nullptr, (T *)C, (long)ldc);
-    bool const fast = direct(A, lda, strideA, TA ? k : m, sizeof(T)) && direct(B, ldb, 0, k, sizeof(T));
     int const tile = product_tile(fast, groups, m, n, (k + 63) / 64);
     auto const launch = fast ? tile == 256 ? gemm_tiles<T, ProductTile<T, 256, 256, 2, 4, TA, true, DIRECT>> : tile == 128 ? gemm_tiles<T, ProductTile<T, 128, 128, 2, 2, TA, true, DIRECT>>
             : gemm_tiles<T, ProductTile<T, 64, 64, 1, 1, TA, true, DIRECT, 4>>
@@ -478,10 +477,10 @@ template <typename T, typename D>
 static hipError_t outer_launch(hipStream_t s, int groups, int m, int n, int k, int const *offsets, void const *X, int ldx, void const *Y, int ldy,
     double beta, void *out, int ldd, long strideD, void *work, long work_size)
 {
-    if (m < 8 || n < 8)
+    bool const fast = direct(X, ldx, 0, sizeof(T)) && direct(Y, ldy, 0, sizeof(T));
+    if (!fast && (m < 8 || n < 8))
         return launch_kernel(grouped_outer_narrow_kernel<T, D>, dim3((unsigned)std::min((long)m * n / 4 + 1, 16384L), 1, groups), 256, s, 0,
             m, n, k, offsets, (T const *)X, (long)ldx, (T const *)Y, (long)ldy, (float)beta, (D *)out, (long)ldd, strideD);
-    bool const fast = direct(X, ldx, 0, m, sizeof(T)) && direct(Y, ldy, 0, n, sizeof(T));
     Cut c = outer_cut(fast, groups, m, n, k);
     long const plane = (long)groups * m * n * 4;
     if (c.slices > 1 && (work == nullptr || work_size < c.slices * plane)) c.slices = 1;
@@ -509,7 +508,6 @@ static int douter_slices(long groups, long m, long n, long k)
 long grouped_outer_work_size(ProductType type, int groups, int m, int n, int k)
 {
     if (type == PRODUCT_F64) { int const slices = douter_slices(groups, m, n, k); return slices > 1 ? (long)slices * groups * m * n * 8 : 0; }
-    if (m < 8 || n < 8) return 0;
     // (whichever way the operands are aligned)
     int const slices = std::max(outer_cut(true, groups, m, n, k).slices, outer_cut(false, groups, m, n, k).slices);
     return slices > 1 ? (long)slices * groups * m * n * 4 : 0;
@@ -574,10 +572,10 @@ static hipError_t gemm_i8_launch(hipStream_t s, int groups, int m, int n, int k,
         };
         return go(gemm_i8_few_kernel<D, 1>, 16);
     }
-    if (k < 16)
+    bool const fast = direct(A, lda, strideA, 1) && direct(B, ldb, 0, 1);
+    if (!fast && k < 16)
         return launch_kernel(grouped_gemm_narrow_kernel<signed char, D>, dim3((unsigned)most_pieces(groups, n, 4), std::min(m, 65535)), 256, s, 0, groups, m, n, k, offsets,
             A, (long)lda, 1L, strideA, scaleA, strideS, B, (long)ldb, scaleB, (D *)C, (long)ldc);
-    bool const fast = direct(A, lda, strideA, k, 1) && direct(B, ldb, 0, k, 1);
     typedef signed char T;
     int const tile = product_tile(fast, groups, m, n, (k + 127) / 128);
     auto const launch = fast ? tile == 256 ? gemm_i8_tiles<D, ProductTile<T, 256, 256, 2, 4, true, true, DIRECT>> : tile == 128 ? gemm_i8_tiles<D, ProductTile<T, 128, 128, 2, 2, true, true, DIRECT>>

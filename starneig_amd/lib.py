@@ -553,14 +553,16 @@ def _product_matrix(name, t, shape, dtype, device):
         return t.data_ptr(), rows, 0
     # (the stride of a dimension of one entry says nothing)
     ld = stride[-2] if shape[-2] > 1 else max(1, rows)
-    if ld < rows:
-        raise ValueError(f"the columns of {name} overlap")
+    if ld < rows or ld > 0x7fffffff:
+        raise ValueError(f"the columns of {name} overlap or lie 2^31 entries apart")
     return t.data_ptr(), ld, (stride[0] if dims == 3 and shape[0] > 1 else 0)
 
 
 def _product_sizes(name, t):
     if t.dim() != 2:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not (columns, rows)")
+    if t.shape[0] > 0x7fffffff:
+        raise ValueError(f"{name} has 2^31 columns or more")
     return t.shape
 
 

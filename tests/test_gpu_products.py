@@ -99,6 +99,11 @@ SIZES = [
     ([1] * 70 + [5, 0, 0, 9] * 20, 96, 72),         # more groups than a wave has lanes
     ([0] * 64 + [3] + [0] * 63 + [40], 40, 136),
     ([1000, 0, 5000, 2100, 77], 2056, 168),         # enough tiles to fill the chip: the large ones
+    ([1000, 0, 5000, 2100, 77], 2058, 42),          # inner lengths that end within a chunk of 8, in the first and the second k-tile
+    ([1000, 0, 5000, 2100, 77], 2058, 108),
+    ([70, 0, 3], 6, 6),
+    ([300], 2, 2),
+    ([200, 30], 130, 204),
 ]
 
 
@@ -213,7 +218,8 @@ def check_outer(S, type_, out, sizes, m, n, beta, first=0, behind=0, pads=(0, 0,
 @pytest.mark.parametrize("sizes,m,n", [
     ([1], 1, 1), ([0, 1, 0], 5, 3), ([33], 64, 64), ([3, 0, 17, 1], 33, 65), ([130, 1, 0, 255, 63], 129, 257), ([700], 256, 96),
     ([257, 513, 5], 300, 512), ([9000], 64, 40), ([20000], 200, 136), ([1] * 70 + [5, 0, 0, 9] * 20, 40, 72), ([4000, 60, 0, 2500], 128, 384),
-    ([100, 0, 333, 64, 1] * 2, 1096, 1544)])
+    ([100, 0, 333, 64, 1] * 2, 1096, 1544),
+    ([100, 0, 333, 64, 1] * 2, 1098, 1546), ([3000, 2], 6, 130), ([300], 2, 2)])
 def test_outer(node, type_, out, beta, sizes, m, n):
     check_outer(node, type_, out, sizes, m, n, beta)
 
@@ -242,7 +248,7 @@ def scaled(sums, scale_row, scale_col, dtype):
 
 @pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (5, 3, 17), (64, 1, 64), (4096, 1, 4096), (1999, 3, 1403), (130, 16, 4096), (257, 33, 129), (300, 130, 640), (512, 512, 1024), (1000, 777, 1403),
-                                   (4112, 4100, 400)])
+                                   (4112, 4100, 400), (4112, 4100, 404), (300, 130, 636), (70, 90, 12)])
 @pytest.mark.parametrize("pad,shift", [(0, 0), (16, 0), (3, 5)])
 def test_gemm_i8(node, out, m, n, k, pad, shift):
     import torch
