@@ -151,7 +151,7 @@ starneig_error_t starneig_amd_dgemm_device(
  * [0, n] counts as the nearer end, one below its predecessor as its predecessor.
  * The calls enqueue on `stream` and return; they hold no state and no lock, so they may run
  * on several streams at once and be captured into graphs.  All pointers are on the current device and aligned to their
- * elements; outputs must not overlap inputs.  Columns aligned to 4 bytes (pointer, leading dimension, stride) are read fastest.
+ * elements; outputs must not overlap inputs; m, n and k are at most 2^30.  Columns aligned to 4 bytes (pointer, leading dimension, stride) are read fastest.
  * fp16 / bf16 sums are held in fp32 and rounded once, fp64 sums as in starneig_amd_dgemm_device; equal calls give
  * equal bits.  A return value of -i marks the i-th argument, STARNEIG_GENERIC_ERROR a launch that failed (sizes beyond
  * 2^32 threads included). */

@@ -950,6 +950,8 @@ SN_API starneig_error_t starneig_amd_dgemm_device(
 namespace {
 int product_size(int type) { return type == STARNEIG_AMD_F64 ? 8 : type == STARNEIG_AMD_F32 ? 4 : type == STARNEIG_AMD_BF16 || type == STARNEIG_AMD_F16 ? 2 : 0; }
 bool bad_pointer(void const *p, int align) { return p == NULL || (uintptr_t)p % align != 0; }
+// rows, columns and inner terms: a tile's further end stays an int
+bool bad_size(int n) { return n < 0 || n > 1 << 30; }
 starneig_error_t launched(hipError_t e) { return e == hipSuccess ? STARNEIG_SUCCESS : STARNEIG_GENERIC_ERROR; }
 }
 
@@ -962,9 +964,9 @@ SN_API starneig_error_t starneig_amd_grouped_gemm_device(
     if (size == 0 || type == STARNEIG_AMD_F32) return -1;
     if (!ta && transA != 'N' && transA != 'n') return -2;
     if (groups < 1) return -3;
-    if (m < 0) return -4;
-    if (n < 0) return -5;
-    if (k < 0) return -6;
+    if (bad_size(m)) return -4;
+    if (bad_size(n)) return -5;
+    if (bad_size(k)) return -6;
     bool const some = m > 0 && n > 0;
     if (some && bad_pointer(dOffsets, 4)) return -7;
     if (some && k > 0 && bad_pointer(dA, size)) return -8;
@@ -988,9 +990,9 @@ SN_API starneig_error_t starneig_amd_grouped_outer_device(
     if (size == 0 || type == STARNEIG_AMD_F32) return -1;
     if (typeD != type && (typeD != STARNEIG_AMD_F32 || type == STARNEIG_AMD_F64)) return -2;
     if (groups < 1 || groups > 65535) return -3;
-    if (m < 0) return -4;
-    if (n < 0) return -5;
-    if (k < 0) return -6;
+    if (bad_size(m)) return -4;
+    if (bad_size(n)) return -5;
+    if (bad_size(k)) return -6;
     bool const some = m > 0 && n > 0;
     if (some && bad_pointer(dOffsets, 4)) return -7;
     if (some && k > 0 && bad_pointer(dX, size)) return -8;
@@ -1011,7 +1013,7 @@ SN_API starneig_error_t starneig_amd_grouped_outer_device(
 
 SN_API long starneig_amd_grouped_outer_work_size(int type, int groups, int m, int n, int k)
 {
-    if (product_size(type) == 0 || type == STARNEIG_AMD_F32 || groups < 1 || groups > 65535 || m < 1 || n < 1 || k < 1) return 0;
+    if (product_size(type) == 0 || type == STARNEIG_AMD_F32 || groups < 1 || groups > 65535 || m < 1 || n < 1 || k < 1 || bad_size(m) || bad_size(n) || bad_size(k)) return 0;
     return sn::grouped_outer_work_size((sn::ProductType)type, groups, m, n, k);
 }
 
@@ -1020,8 +1022,8 @@ SN_API starneig_error_t starneig_amd_quantize_i8_device(
 {
     int const size = product_size(type);
     if (size == 0 || type == STARNEIG_AMD_F64) return -1;
-    if (k < 0) return -2;
-    if (n < 0) return -3;
+    if (bad_size(k)) return -2;
+    if (bad_size(n)) return -3;
     if (n > 0 && k > 0 && bad_pointer(dX, size)) return -4;
     if (ldX < std::max(1, k)) return -5;
     if (n > 0 && k > 0 && bad_pointer(dQ, 1)) return -6;
@@ -1038,8 +1040,8 @@ SN_API starneig_error_t starneig_amd_gemm_i8_device(
 {
     int const size = product_size(typeC);
     if (size == 0 || typeC == STARNEIG_AMD_F64) return -1;
-    if (m < 0) return -2;
-    if (n < 0) return -3;
+    if (bad_size(m)) return -2;
+    if (bad_size(n)) return -3;
     if (k < 0 || k > 131071) return -4;         // 131071 * 128 * 128 < 2^31
     bool const some = m > 0 && n > 0;
     if (some && k > 0 && bad_pointer(dA, 1)) return -5;
@@ -1063,8 +1065,8 @@ SN_API starneig_error_t starneig_amd_grouped_gemm_i8_device(
     int const size = product_size(typeC);
     if (size == 0 || typeC == STARNEIG_AMD_F64) return -1;
     if (groups < 1) return -2;
-    if (m < 0) return -3;
-    if (n < 0) return -4;
+    if (bad_size(m)) return -3;
+    if (bad_size(n)) return -4;
     if (k < 0 || k > 131071) return -5;
     bool const some = m > 0 && n > 0;
     if (some && bad_pointer(dOffsets, 4)) return -6;
