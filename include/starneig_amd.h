@@ -151,7 +151,8 @@ starneig_error_t starneig_amd_dgemm_device(
  * [0, n] counts as the nearer end, one below its predecessor as its predecessor.
  * The calls enqueue on `stream` and return; they hold no state and no lock, so they may run
  * on several streams at once and be captured into graphs.  All pointers are on the current device and aligned to their
- * elements; outputs must not overlap inputs; m, n and k are at most 2^30.  Columns aligned to 4 bytes (pointer, leading dimension, stride) are read fastest.
+ * elements; outputs must not overlap inputs; m, n and k are at most 2^30, groups
+ * 65535.  Columns aligned to 4 bytes (pointer, leading dimension, stride) are read fastest.
  * fp16 / bf16 sums are held in fp32 and rounded once, fp64 sums as in starneig_amd_dgemm_device; equal calls give
  * equal bits.  A return value of -i marks the i-th argument, STARNEIG_GENERIC_ERROR a launch that failed (sizes beyond
  * 2^32 threads included). */
@@ -167,7 +168,7 @@ starneig_error_t starneig_amd_grouped_gemm_device(
 
 /* D_g = X_g Y_g^T + beta D_g, the sum over the columns of group g: the gradient of A_g with X = B and Y = the gradient
  * of C (transA = 'T'), or X and Y swapped ('N').  X: m x k, Y: n x k (k: all columns), D_g: m x n at dD + g strideD
- * elements.  An empty group gives beta D_g; beta = 0 does not read D.  typeD: `type`, or F32 for BF16 / F16.  At most 65535 groups.
+ * elements.  An empty group gives beta D_g; beta = 0 does not read D.  typeD: `type`, or F32 for BF16 / F16.
  * dWork: scratch memory of the call's own (two captured graphs that may run at once need two), 16-byte aligned, of workSize bytes.  With
  * starneig_amd_grouped_outer_work_size bytes of it a long sum over few outputs is cut into parts that run at once; with less, or NULL, it is
  * not cut: slower, and rounded differently. */
@@ -179,7 +180,7 @@ starneig_error_t starneig_amd_grouped_outer_device(
 long starneig_amd_grouped_outer_work_size(int type, int groups, int m, int n, int k);
 
 /* Q(:, c) = rint(X(:, c) / s_c), s_c = dScale[c] = max_i |X(i, c)| / 127 in IEEE fp32, halves to even.  X: k x n of type F32, BF16 or F16.
- * A column of zeros gets s = 0 and Q = 0; one that holds an infinity or a NaN gets that s and Q = 0 (its product is NaN). */
+ * A column of zeros (or whose s underflows to 0) gets s = 0 and Q = 0; one that holds an infinity or a NaN gets that s and Q = 0 (its product is NaN). */
 starneig_error_t starneig_amd_quantize_i8_device(
     int type, int k, int n, void const *dX, int ldX, signed char *dQ, int ldQ, float *dScale, void *stream);
 

@@ -952,6 +952,8 @@ int product_size(int type) { return type == STARNEIG_AMD_F64 ? 8 : type == STARN
 bool bad_pointer(void const *p, int align) { return p == NULL || (uintptr_t)p % align != 0; }
 // rows, columns and inner terms: a tile's further end stays an int
 bool bad_size(int n) { return n < 0 || n > 1 << 30; }
+// (every tile walks over the groups)
+bool bad_groups(int groups) { return groups < 1 || groups > 65535; }
 starneig_error_t launched(hipError_t e) { return e == hipSuccess ? STARNEIG_SUCCESS : STARNEIG_GENERIC_ERROR; }
 }
 
@@ -963,7 +965,7 @@ SN_API starneig_error_t starneig_amd_grouped_gemm_device(
     int const size = product_size(type);
     if (size == 0 || type == STARNEIG_AMD_F32) return -1;
     if (!ta && transA != 'N' && transA != 'n') return -2;
-    if (groups < 1) return -3;
+    if (bad_groups(groups)) return -3;
     if (bad_size(m)) return -4;
     if (bad_size(n)) return -5;
     if (bad_size(k)) return -6;
@@ -989,7 +991,7 @@ SN_API starneig_error_t starneig_amd_grouped_outer_device(
     int const size = product_size(type);
     if (size == 0 || type == STARNEIG_AMD_F32) return -1;
     if (typeD != type && (typeD != STARNEIG_AMD_F32 || type == STARNEIG_AMD_F64)) return -2;
-    if (groups < 1 || groups > 65535) return -3;
+    if (bad_groups(groups)) return -3;
     if (bad_size(m)) return -4;
     if (bad_size(n)) return -5;
     if (bad_size(k)) return -6;
@@ -1013,7 +1015,7 @@ SN_API starneig_error_t starneig_amd_grouped_outer_device(
 
 SN_API long starneig_amd_grouped_outer_work_size(int type, int groups, int m, int n, int k)
 {
-    if (product_size(type) == 0 || type == STARNEIG_AMD_F32 || groups < 1 || groups > 65535 || m < 1 || n < 1 || k < 1 || bad_size(m) || bad_size(n) || bad_size(k)) return 0;
+    if (product_size(type) == 0 || type == STARNEIG_AMD_F32 || bad_groups(groups) || m < 1 || n < 1 || k < 1 || bad_size(m) || bad_size(n) || bad_size(k)) return 0;
     return sn::grouped_outer_work_size((sn::ProductType)type, groups, m, n, k);
 }
 
@@ -1064,7 +1066,7 @@ SN_API starneig_error_t starneig_amd_grouped_gemm_i8_device(
 {
     int const size = product_size(typeC);
     if (size == 0 || typeC == STARNEIG_AMD_F64) return -1;
-    if (groups < 1) return -2;
+    if (bad_groups(groups)) return -2;
     if (bad_size(m)) return -3;
     if (bad_size(n)) return -4;
     if (k < 0 || k > 131071) return -5;

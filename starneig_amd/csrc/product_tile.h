@@ -155,7 +155,6 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
         #pragma unroll
         for (int s = 0; s < O::LOADS; s++) load(lds, s);
     }
-    __device__ __forceinline__ void put(lds_char *, int, int) const {}
 };
 
 // 16 bytes of global memory from any address

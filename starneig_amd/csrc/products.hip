@@ -82,11 +82,11 @@ void grouped_outer_kernel(int groups, int m, int n, int k, int slices, int const
     int const rows = (m + P::BM - 1) / P::BM, cols = (n + P::BN - 1) / P::BN, each = rows * cols, items = groups * slices * each;
     Longest order(offsets, groups, k);
     P tile;
-    struct Place { int group, slice; bool there; };
+    struct Item { int group, slice; bool there; };
     tile.all(lds, [&](int turn, Plan<T> &p) {
         int const here = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
         unsigned const i = turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - here : here);
-        if (i >= (unsigned)items) return Place{0, 0, false};
+        if (i >= (unsigned)items) return Item{0, 0, false};
         Span const s = order.at(i / (unsigned)(each * slices));
         int const in = i % (unsigned)(each * slices), slice = (unsigned)in / (unsigned)each;
         int row, col;
@@ -95,8 +95,8 @@ void grouped_outer_kernel(int groups, int m, int n, int k, int slices, int const
         int const begin = s.begin + (int)min((long)slice * part, (long)length), end = min(begin + part, s.end);
         int const r0 = row * P::BM, c0 = col * P::BN;
         p = Plan<T>{X + begin * ldx + r0, Y + begin * ldy + c0, ldx, ldy, m - r0, n - c0, end - begin, r0, c0};
-        return Place{s.group, slice, true};
-    }, [&](Plan<T> const &p, Place const &at) {
+        return Item{s.group, slice, true};
+    }, [&](Plan<T> const &p, Item const &at) {
         Columns<D> const to{out + ((long)at.slice * groups + at.group) * strideD + p.c0 * ldd + p.r0, ldd, p.rows, p.cols};
         if (beta == 0.f) tile.template store<D>(lds, [&](int x, int t, int y, int u, int r) { return (D)tile.acc[x][t][y][u][r]; }, to);
         else tile.template store<float>(lds, [&](int x, int t, int y, int u, int r) { return tile.acc[x][t][y][u][r]; }, Added<D>{to, beta});
@@ -212,52 +212,43 @@ void grouped_outer_narrow_kernel(int m, int n, int k, int const *__restrict__ of
 }
 
 // Few columns a group (a token or a batch of them while text is generated): the matrix is read once, as fast as memory gives it, and nothing
-// else counts.  A workgroup takes 16 rows of A_g and up to 16 NT columns; its eight waves cut the inner index into eight runs, load their operands
+// else counts.  A workgroup takes 16 rows of A_g and up to 16 columns; its eight waves cut the inner index into eight runs, load their operands
 // straight into the matrix instructions' registers, eight 16-byte loads of A in flight a lane, and add up their
 // sums through LDS in the waves' order.  Only for A with the inner index contiguous.  Any alignment: the chunk that k cuts is
 // read from where it ends at k, and what of it the chunk before held is zeroed, in both operands alike.
 // One token through 8 of 64 matrices 1024 x 2048 in bf16: 9.5 us, 3.5 TB/s; 4096 x 4096 in 8 bits: 5.3 us, 3.2 TB/s.
-template <typename T, int NT, typename Out>
+template <typename T, typename Out>
 __device__ __forceinline__ void few_columns_tile(T const *__restrict__ A, long lda, int rows, T const *__restrict__ B, long ldb, int cols, int k, Out &&out)
 {
     constexpr int EL = 16 / (int)sizeof(T), WAVES = 8, U = 8;
     typedef typename Mfma<T>::Acc16 Acc;
-    __shared__ __attribute__((aligned(16))) Acc sums[WAVES][NT][64];
+    __shared__ __attribute__((aligned(16))) Acc sums[WAVES][64];
     int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     int const steps = (k + 4 * EL - 1) / (4 * EL), run = (steps + WAVES - 1) / WAVES;
     int const first = min(wave * run, steps), end = min(first + run, steps);
     T const *const a = A + min(i, rows - 1) * lda;          // (a row or column that is not there: another's, and its result is not stored)
-    T const *b[NT];
-    #pragma unroll
-    for (int t = 0; t < NT; t++) b[t] = B + min(16 * t + i, cols - 1) * ldb;
-    Acc acc[NT];
-    #pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = Acc{};
+    T const *const b = B + min(i, cols - 1) * ldb;
+    Acc acc = {};
     // chunk q of step s: entirely below k in all but the last step
     int s = first;
     for (; s + U <= min(end, k / (4 * EL)); s += U) {
-        i32x4 va[U], vb[U][NT];
+        i32x4 va[U], vb[U];
         #pragma unroll
         for (int u = 0; u < U; u++) va[u] = load16(a + ((s + u) * 4 + q) * EL);
         #pragma unroll
-        for (int u = 0; u < U; u++)
-            #pragma unroll
-            for (int t = 0; t < NT; t++) vb[u][t] = load16(b[t] + ((s + u) * 4 + q) * EL);
+        for (int u = 0; u < U; u++) vb[u] = load16(b + ((s + u) * 4 + q) * EL);
         #pragma unroll
-        for (int u = 0; u < U; u++)
-            #pragma unroll
-            for (int t = 0; t < NT; t++) acc[t] = Mfma<T>::mul16(va[u], vb[u][t], acc[t]);
+        for (int u = 0; u < U; u++) acc = Mfma<T>::mul16(va[u], vb[u], acc);
     }
     if (s < end) {
-        i32x4 va[U], vb[U][NT];
+        i32x4 va[U], vb[U];
         int skip[U];
         #pragma unroll
         for (int u = 0; u < U; u++) {
             int const at = ((s + u) * 4 + q) * EL, from = min(at, k - EL);
             skip[u] = s + u < end ? min(at - from, EL) : EL;
             va[u] = load16(a + from);
-            #pragma unroll
-            for (int t = 0; t < NT; t++) vb[u][t] = load16(b[t] + from);
+            vb[u] = load16(b + from);
         }
         #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -268,40 +259,38 @@ __device__ __forceinline__ void few_columns_tile(T const *__restrict__ A, long l
                 mask[w] = bits == 32 ? 0 : (int)(0xffffffffu << bits);
             }
             va[u] &= mask;
-            #pragma unroll
-            for (int t = 0; t < NT; t++) acc[t] = Mfma<T>::mul16(va[u], vb[u][t] & mask, acc[t]);
+            acc = Mfma<T>::mul16(va[u], vb[u] & mask, acc);
         }
     }
-    #pragma unroll
-    for (int t = 0; t < NT; t++) sums[wave][t][lane] = acc[t];
+    sums[wave][lane] = acc;
     __syncthreads();
     // lane l, register r of a sum is row 4 (l >> 4) + r, column l & 15
-    for (int e = threadIdx.x; e < 256 * NT; e += 64 * WAVES) {
-        int const row = e & 15, col = e >> 4, l = (row >> 2) * 16 + (col & 15);
-        auto sum = sums[0][col >> 4][l][row & 3];
+    if (threadIdx.x < 256) {
+        int const row = threadIdx.x & 15, col = threadIdx.x >> 4, l = (row >> 2) * 16 + col;
+        auto sum = sums[0][l][row & 3];
         #pragma unroll
-        for (int w = 1; w < WAVES; w++) sum += sums[w][col >> 4][l][row & 3];
+        for (int w = 1; w < WAVES; w++) sum += sums[w][l][row & 3];
         if (row < rows && col < cols) out(row, col, sum);
     }
 }
 
-template <typename T, int NT>
+template <typename T>
 __global__ __launch_bounds__(512)
 void grouped_gemm_few_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, T const *__restrict__ A, long lda, long strideA,
     T const *__restrict__ B, long ldb, T *__restrict__ C, long ldc)
 {
-    Pieces pieces(offsets, groups, n, 16 * NT);
+    Pieces pieces(offsets, groups, n, 16);
     int const t = tile_of_workgroup((m + 15) / 16 * pieces.total, 0);
     if (t < 0) return;
     Span const s = pieces.at((unsigned)t % (unsigned)pieces.total);
     int const row = (unsigned)t / (unsigned)pieces.total;
     int const r0 = row * 16;
-    few_columns_tile<T, NT>(A + s.group * strideA + r0 * lda, lda, m - r0, B + s.begin * ldb, ldb, s.end - s.begin, k,
+    few_columns_tile<T>(A + s.group * strideA + r0 * lda, lda, m - r0, B + s.begin * ldb, ldb, s.end - s.begin, k,
         [&](int r, int c, float sum) { C[(s.begin + c) * ldc + r0 + r] = (T)sum; });
 }
 
 // fp64: the tile of the library's own dgemm, one piece of a group a workgroup; the tile rows of a piece side by side, so that its columns
-// come from memory once (24 matrices 312 x 312, 40000 columns: 182 us, 43 TFLOP/s; 20000 columns, 8 matrices 1024 x 1024: 757 us, 55 TFLOP/s)
+// come from memory once (24 matrices 312 x 312, 40000 columns: 170 us, 46 TFLOP/s; 20000 columns, 8 matrices 1024 x 1024: 757 us, 55 TFLOP/s)
 template <bool TA>
 __global__ __launch_bounds__(256, 2)
 void grouped_dgemm_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, double const *__restrict__ A, int lda, long strideA,
@@ -418,11 +407,8 @@ static hipError_t gemm_launch(hipStream_t s, int groups, int m, int n, int k, in
     void const *B, int ldb, void *C, int ldc)
 {
     if (TA && k >= 8 && few_columns(groups, m, n)) {
-        auto const go = [&](auto kernel, int width) {
-            return launch_kernel(kernel, dim3((unsigned)roundup(most_pieces(groups, n, width) * ((m + 15) / 16), 8)), 512, s, 0,
-                groups, m, n, k, offsets, (T const *)A, (long)lda, strideA, (T const *)B, (long)ldb, (T *)C, (long)ldc);
-        };
-        return go(grouped_gemm_few_kernel<T, 1>, 16);
+        return launch_kernel(grouped_gemm_few_kernel<T>, dim3((unsigned)roundup(most_pieces(groups, n, 16) * ((m + 15) / 16), 8)), 512, s, 0,
+            groups, m, n, k, offsets, (T const *)A, (long)lda, strideA, (T const *)B, (long)ldb, (T *)C, (long)ldc);
     }
     bool const fast = direct(A, lda, strideA, sizeof(T)) && direct(B, ldb, 0, sizeof(T));
     if (!fast && (k < 8 || (!TA && m < 8)))
@@ -535,19 +521,19 @@ hipError_t grouped_outer(hipStream_t s, ProductType type, ProductType typeD, int
 
 // ---- 8-bit integers ----------------------------------------------------------------------------------------------
 
-template <typename D, int NT>
+template <typename D>
 __global__ __launch_bounds__(512)
 void gemm_i8_few_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, signed char const *__restrict__ A, long lda, long strideA,
     float const *__restrict__ scaleA, long strideS, signed char const *__restrict__ B, long ldb, float const *__restrict__ scaleB, D *__restrict__ C, long ldc)
 {
-    Pieces pieces(offsets, groups, n, 16 * NT);
+    Pieces pieces(offsets, groups, n, 16);
     int const t = tile_of_workgroup((m + 15) / 16 * pieces.total, 0);
     if (t < 0) return;
     Span const s = pieces.at((unsigned)t % (unsigned)pieces.total);
     int const row = (unsigned)t / (unsigned)pieces.total;
     int const r0 = row * 16;
     float const *const sa = scaleA + s.group * strideS + r0;
-    few_columns_tile<signed char, NT>(A + s.group * strideA + r0 * lda, lda, m - r0, B + s.begin * ldb, ldb, s.end - s.begin, k,
+    few_columns_tile<signed char>(A + s.group * strideA + r0 * lda, lda, m - r0, B + s.begin * ldb, ldb, s.end - s.begin, k,
         [&](int r, int c, int sum) { C[(s.begin + c) * ldc + r0 + r] = (D)scaled(sum, sa[r], scaleB[s.begin + c]); });
 }
 
@@ -566,11 +552,8 @@ static hipError_t gemm_i8_launch(hipStream_t s, int groups, int m, int n, int k,
     float const *scaleA, long strideS, signed char const *B, int ldb, float const *scaleB, void *C, int ldc)
 {
     if (k >= 16 && few_columns(groups, m, n)) {
-        auto const go = [&](auto kernel, int width) {
-            return launch_kernel(kernel, dim3((unsigned)roundup(most_pieces(groups, n, width) * ((m + 15) / 16), 8)), 512, s, 0,
-                groups, m, n, k, offsets, A, (long)lda, strideA, scaleA, strideS, B, (long)ldb, scaleB, (D *)C, (long)ldc);
-        };
-        return go(gemm_i8_few_kernel<D, 1>, 16);
+        return launch_kernel(gemm_i8_few_kernel<D>, dim3((unsigned)roundup(most_pieces(groups, n, 16) * ((m + 15) / 16), 8)), 512, s, 0,
+            groups, m, n, k, offsets, A, (long)lda, strideA, scaleA, strideS, B, (long)ldb, scaleB, (D *)C, (long)ldc);
     }
     bool const fast = direct(A, lda, strideA, 1) && direct(B, ldb, 0, 1);
     if (!fast && k < 16)

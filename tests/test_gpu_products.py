@@ -643,3 +643,51 @@ def test_refusals_on_the_gpu(node):
     with pytest.raises(ValueError):
         node.gemm_i8_device(A[0].char(), torch.zeros(5, device="cuda"), B.char(), torch.zeros(4, device="cuda"), C)
     assert node.gemm_i8_device(A[0].char(), torch.zeros(6, device="cuda"), B.char(), torch.zeros(4, device="cuda"), C.double()) == -1
+
+
+@pytest.mark.parametrize("type_", TYPES)
+def test_the_most_groups(node, type_):
+    """65535 groups, nearly all empty: the products of the few columns, and zeros or beta D from the others."""
+    import torch
+    gen, dtype, groups, m, n, k = generator(71), kind(type_), 65535, 24, 9, 40
+    sizes = np.zeros(groups, dtype=int)
+    filled = {0: 2, 63: 1, 64: 3, 40000: 17, groups - 1: 20}
+    for g, size in filled.items():
+        sizes[g] = size
+    total = sum(filled.values())
+    A = padded(gen, 1, m, k, dtype=dtype)
+    B, C = padded(gen, total, k, dtype=dtype), padded(gen, total, m, dtype=dtype)
+    assert node.grouped_gemm_device("T", offsets_of(sizes), A.expand(groups, m, k), B, C) == 0
+    a, b = A[0].double().T, B.double()
+    ref = b @ a
+    assert bool(((C.double() - ref).abs() <= product_bound(k, b.abs() @ a.abs(), ref, dtype)).all())
+    X, Y = padded(gen, total, m, dtype=dtype), padded(gen, total, n, dtype=dtype)
+    D = torch.full((groups, n, m), 3.0, dtype=dtype, device="cuda")
+    assert node.grouped_outer_device(offsets_of(sizes), X, Y, D, beta=0.5) == 0
+    at = 0
+    for g, size in filled.items():
+        x, y = X[at:at + size].double(), Y[at:at + size].double()
+        ref = y.T.contiguous() @ x + 1.5
+        bound = product_bound(size + 2, y.abs().T.contiguous() @ x.abs() + 1.5, ref, dtype)
+        assert bool(((D[g].double() - ref).abs() <= bound).all()), g
+        at += size
+    empty = torch.ones(groups, dtype=torch.bool, device="cuda")
+    empty[list(filled)] = False
+    assert bool((D[empty] == 1.5).all())
+
+
+@pytest.mark.parametrize("tokens", [1, 50])
+def test_8_bit_groups_that_share_their_scales(node, tokens):
+    """One matrix and one row of scales for all groups (strides of zero), some groups without a column."""
+    import torch
+    gen, groups, m, k = generator(73), 5, 130, 264
+    sizes = [0, tokens, 0, 2, tokens]
+    n = sum(sizes)
+    A, B = whole(gen, 1, m, k), whole(gen, n, k)
+    sa, sb = torch.rand(1, m, generator=gen, device="cuda"), torch.rand(n, generator=gen, device="cuda")
+    C = torch.empty(n, m, dtype=torch.float32, device="cuda")
+    assert node.load().starneig_amd_grouped_gemm_i8_device(
+        node.AMD_F32, groups, m, n, k, offsets_of(sizes).data_ptr(), A.data_ptr(), k, 0, sa.data_ptr(), 0, B.data_ptr(), k, sb.data_ptr(), C.data_ptr(), m,
+        torch.cuda.current_stream().cuda_stream) == 0
+    sums = B.double() @ A[0].double().T.contiguous()
+    assert torch.equal(C, scaled(sums, sa[0], sb, torch.float32))

@@ -23,7 +23,7 @@ BIG = (1 << 30) + 1
 
 REFUSED = [
     ("grouped_gemm_device", GEMM, [
-        (1, dict(type=S.AMD_F32)), (1, dict(type=7)), (1, dict(type=-1)), (2, dict(trans=b"C")), (3, dict(groups=0)), (4, dict(m=-1)), (5, dict(n=-1)),
+        (1, dict(type=S.AMD_F32)), (1, dict(type=7)), (1, dict(type=-1)), (2, dict(trans=b"C")), (3, dict(groups=0)), (3, dict(groups=65536)), (4, dict(m=-1)), (5, dict(n=-1)),
         (6, dict(k=-1)), (4, dict(m=BIG)), (5, dict(n=BIG)), (6, dict(k=BIG)), (7, dict(off=None)), (7, dict(off=P + 2)), (8, dict(A=None)), (8, dict(A=P + 1)), (9, dict(ldA=15)), (9, dict(trans=b"N", ldA=7)),
         (10, dict(strideA=-1)), (11, dict(B=None)), (11, dict(B=P + 1)), (12, dict(ldB=15)), (13, dict(C=None)), (13, dict(C=P + 1)), (14, dict(ldC=7))]),
     ("grouped_outer_device", OUTER, [
@@ -37,7 +37,7 @@ REFUSED = [
         (1, dict(typeC=S.AMD_F64)), (2, dict(m=-1)), (3, dict(n=-1)), (2, dict(m=BIG)), (3, dict(n=BIG)), (4, dict(k=-1)), (4, dict(k=131072, ldA=131072, ldB=131072)), (5, dict(A=None)), (6, dict(ldA=15)),
         (7, dict(sA=None)), (7, dict(sA=P + 1)), (8, dict(B=None)), (9, dict(ldB=15)), (10, dict(sB=None)), (11, dict(C=None)), (11, dict(C=P + 1)), (12, dict(ldC=7))]),
     ("grouped_gemm_i8_device", GI8, [
-        (1, dict(typeC=S.AMD_F64)), (2, dict(groups=0)), (3, dict(m=-1)), (4, dict(n=-1)), (3, dict(m=BIG)), (4, dict(n=BIG)), (5, dict(k=-1)), (5, dict(k=131072, ldA=131072, ldB=131072)), (6, dict(off=None)), (7, dict(A=None)),
+        (1, dict(typeC=S.AMD_F64)), (2, dict(groups=0)), (2, dict(groups=65536)), (3, dict(m=-1)), (4, dict(n=-1)), (3, dict(m=BIG)), (4, dict(n=BIG)), (5, dict(k=-1)), (5, dict(k=131072, ldA=131072, ldB=131072)), (6, dict(off=None)), (7, dict(A=None)),
         (8, dict(ldA=15)), (9, dict(strideA=-1)), (10, dict(sA=None)), (11, dict(strideS=-1)), (12, dict(B=None)), (13, dict(ldB=15)), (14, dict(sB=None)),
         (15, dict(C=None)), (15, dict(C=P + 1)), (16, dict(ldC=7))]),
 ]
