@@ -54,8 +54,8 @@ struct Operand {
     static constexpr int CR = ROWS / EL;                    // MN: chunks a row
 
     // (ds_read_b128 serves 16 lanes at a time: 0-3, 12-15, 20-27; 4-11, 16-19, 28-31; and so on; ds_read_b64_tr_b16 32)
-    static __device__ __forceinline__ int swizzle_k(int r) { return (r >> 1 & 1) | (r >> 3 & 6); }
-    static __device__ __forceinline__ int swizzle_mn(int k) { return CR >= 16 ? (k & 3) << 2 : (k & 2) << 1; }
+    static __device__ __forceinline__ int swizzle_k(int r) { return sizeof(T) == 8 ? r >> 1 & 7 : (r >> 1 & 1) | (r >> 3 & 6); }
+    static __device__ __forceinline__ int swizzle_mn(int k) { return sizeof(T) == 8 ? 0 : CR >= 16 ? (k & 3) << 2 : (k & 2) << 1; }
 
     // row of lane i of fragment t of 64 rows
     static __device__ __forceinline__ int row(int i, int t) { return K ? 8 * (i >> 2) + 4 * t + (i & 3) : 32 * t + i; }
@@ -79,6 +79,23 @@ struct Operand {
         for (int r = thread_now() % THREADS; r < ROWS; r += THREADS) {
             lds_i32x4 *const at = (lds_i32x4 *)(lds + r * 128 + ((left / EL ^ swizzle_k(r)) << 4));
             *at = *at & mask;
+        }
+    }
+
+    // fp64: the fragments t of 32 rows from `row0` for two instructions e, which take the inner terms 8 half + 2 q + e of the lanes with q = lane >> 4: two
+    // 16-byte reads, of two inner terms (K) or of the two fragments' rows (MN) each
+    static __device__ __forceinline__ int double_row(int i, int t) { return K ? 16 * t + i : 2 * i + t; }
+    static __device__ __forceinline__ void doubles(lds_char const *lds, int row0, int half, double (&f)[2][2])
+    {
+        typedef double d2 __attribute__((ext_vector_type(2)));
+        typedef __attribute__((address_space(3))) d2 lds_d2;
+        int const lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+        #pragma unroll
+        for (int x = 0; x < 2; x++) {
+            int const r = row0 + 16 * x + i, k = 8 * half + 2 * q + x;
+            d2 const v = *(lds_d2 const *)(K ? lds + r * 128 + ((4 * half + q ^ swizzle_k(r)) << 4) : lds + k * (ROWS * 8) + (row0 / 2 + i) * 16);
+            (K ? f[0][x] : f[x][0]) = v.x;
+            (K ? f[1][x] : f[x][1]) = v.y;
         }
     }
 
@@ -517,6 +534,94 @@ struct ProductTile {
                             out.template put<WHOLE>(m0 + 64 * x + 32 * half + (lane & 7) * EL, n0 + 64 * y + OB::row((lane >> 3) + 8 * i, u), v);
                         }
                     }
+    }
+};
+
+// 64 x 64 outputs in fp64, four waves of 32 x 32.  A k-tile is 16 inner terms; LDS holds three of both operands, fed directly, so that a k-tile's loads
+// have two k-tiles' time, and there is one barrier a k-tile; three workgroups a compute unit hide what is left.  Like in the
+// library's dgemm, sums of 256 terms are added up in their turn.
+template <bool AK, bool BK>
+struct DoubleTile {
+    static constexpr int SIZE = 64, THREADS = 256, FLUSH = 16;
+    using SA = Stream<double, SIZE, AK, THREADS, DIRECT>;
+    using SB = Stream<double, SIZE, BK, THREADS, DIRECT>;
+    using OA = typename SA::O;
+    using OB = typename SB::O;
+    static constexpr int KT = OA::KT, PLACE = OA::BYTES, PAIR = 2 * PLACE, LDS_BYTES = 3 * PAIR;
+    typedef double d4 __attribute__((ext_vector_type(4)));
+
+    d4 sum[2][2];           // [columns][rows]: lane l, register r: row l & 15, column (l >> 4) + 4 r of the fragments'
+
+    // p.k may be 0
+    __device__ __forceinline__ void run(Plan<double> const &p, char *shared)
+    {
+        lds_char *const lds = (lds_char *)shared;
+        int const wave = wave_number(), m0 = wave % 2 * 32, n0 = wave / 2 * 32;
+        int const lds0 = uniform((int)(unsigned long long)lds), tiles = (p.k + KT - 1) / KT, cut = (AK || BK) && p.k % OA::EL != 0 ? p.k / KT : -1;
+        SA a;
+        SB b;
+        a.set(p.A, p.rows, p.k, p.lda); b.set(p.B, p.cols, p.k, p.ldb);
+        #pragma unroll
+        for (int i = 0; i < 2; i++) { a.fetch(lds0 + i * PAIR, i); b.fetch(lds0 + i * PAIR + PLACE, i); }
+        d4 acc[2][2];
+        #pragma unroll
+        for (int c = 0; c < 2; c++)
+            #pragma unroll
+            for (int r = 0; r < 2; r++) acc[c][r] = sum[c][r] = d4{0.0, 0.0, 0.0, 0.0};
+        int now = 0;
+        for (int kt = 0; kt < tiles; kt++) {
+            // this k-tile is there, and every wave has read the one before, whose place the next loads take
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(OA::LOADS + OB::LOADS) : "memory");
+            if (kt == cut) {
+                if (AK) OA::trim(lds + now, p.k % KT);
+                if (BK) OB::trim(lds + now + PLACE, p.k % KT);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+            int const free = now == 0 ? 2 * PAIR : now - PAIR;
+            a.fetch(lds0 + free, kt + 2); b.fetch(lds0 + free + PLACE, kt + 2);
+            double fa[2][2][2], fb[2][2][2];
+            #pragma unroll
+            for (int h = 0; h < 2; h++) { OA::doubles(lds + now, m0, h, fa[h]); OB::doubles(lds + now + PLACE, n0, h, fb[h]); }
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                __builtin_amdgcn_sched_barrier(0);
+                #pragma unroll
+                for (int e = 0; e < 2; e++)
+                    #pragma unroll
+                    for (int c = 0; c < 2; c++)
+                        #pragma unroll
+                        for (int r = 0; r < 2; r++) acc[c][r] = __builtin_amdgcn_mfma_f64_16x16x4f64(fb[h][e][c], fa[h][e][r], acc[c][r], 0, 0, 0);
+            }
+            if ((kt + 1) % FLUSH == 0)
+                #pragma unroll
+                for (int c = 0; c < 2; c++)
+                    #pragma unroll
+                    for (int r = 0; r < 2; r++) { sum[c][r] += acc[c][r]; acc[c][r] = d4{0.0, 0.0, 0.0, 0.0}; }
+            now = now == 2 * PAIR ? 0 : now + PAIR;
+        }
+        #pragma unroll
+        for (int c = 0; c < 2; c++)
+            #pragma unroll
+            for (int r = 0; r < 2; r++) sum[c][r] += acc[c][r];
+        // (what was fetched past the end is zeros that nobody reads, but it must have landed before LDS is another workgroup's)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    // C = sums + beta C, of which rows x cols exist
+    __device__ __forceinline__ void store(double beta, double *C, long ldc, int rows, int cols) const
+    {
+        int const lane = threadIdx.x & 63, wave = wave_number(), m0 = wave % 2 * 32, n0 = wave / 2 * 32;
+        #pragma unroll
+        for (int c = 0; c < 2; c++)
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                int const col = n0 + OB::double_row((lane >> 4) + 4 * i, c);
+                #pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    int const row = m0 + OA::double_row(lane & 15, r);
+                    double *const to = C + col * ldc + row;
+                    if (col < cols && row < rows) *to = beta == 0.0 ? sum[c][r][i] : fma(beta, *to, sum[c][r][i]);
+                }
+            }
     }
 };
 

@@ -289,10 +289,11 @@ void grouped_gemm_few_kernel(int groups, int m, int n, int k, int const *__restr
         [&](int r, int c, float sum) { C[(s.begin + c) * ldc + r0 + r] = (T)sum; });
 }
 
-// fp64: the tile of the library's own dgemm, one piece of a group a workgroup; the tile rows of a piece side by side, so that its columns
-// come from memory once (24 matrices 312 x 312, 40000 columns: 170 us, 46 TFLOP/s; 20000 columns, 8 matrices 1024 x 1024: 757 us, 55 TFLOP/s)
-template <bool TA>
-__global__ __launch_bounds__(256, 2)
+// fp64: one piece of a group a workgroup; the tile rows of a piece side by side, so that its columns come from memory once.
+// FAST: operands that can be fed directly; others by the tile of the library's own dgemm.
+// (24 matrices 312 x 312, 40000 columns: 154 us, 51 TFLOP/s, with the tile of dgemm 172 us; 20000 columns, 8 matrices 1024 x 1024: 705 us, 60 TFLOP/s, 762 us)
+template <bool TA, bool FAST>
+__global__ __launch_bounds__(256, FAST ? 3 : 2)
 void grouped_dgemm_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, double const *__restrict__ A, int lda, long strideA,
     double const *__restrict__ B, int ldb, double *__restrict__ C, int ldc)
 {
@@ -301,19 +302,20 @@ void grouped_dgemm_kernel(int groups, int m, int n, int k, int const *__restrict
     if (t < 0) return;
     int const row = (unsigned)t % (unsigned)rows;
     Span const s = pieces.at((unsigned)t / (unsigned)rows);
-    if (k == 0) {           // (the tile reads its operands' last inner term: there must be one)
-        for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-            int const r = row * 64 + e % 64, c = s.begin + e / 64;
-            if (r < m && c < s.end) C[(size_t)c * ldc + r] = 0.0;
-        }
-        return;
-    }
-    gemm_tile<64, 64, 16, TA, false, 16>(m, s.end - s.begin, k, 1.0, A + s.group * strideA, lda, B + (size_t)s.begin * ldb, ldb,
-        0.0, C + (size_t)s.begin * ldc, ldc, row, 0);
+    if constexpr (FAST) {
+        __shared__ __attribute__((aligned(16))) char lds[DoubleTile<TA, true>::LDS_BYTES];
+        long const r0 = row * 64;
+        DoubleTile<TA, true> tile;
+        tile.run(Plan<double>{A + s.group * strideA + r0 * (TA ? lda : 1), B + (long)s.begin * ldb, lda, ldb, m - row * 64, s.end - s.begin, k, 0, 0}, lds);
+        tile.store(0.0, C + (long)s.begin * ldc + r0, ldc, m - row * 64, s.end - s.begin);
+    } else          // (k > 0: this tile reads its operands' last inner term)
+        gemm_tile<64, 64, 16, TA, false, 16>(m, s.end - s.begin, k, 1.0, A + s.group * strideA, lda, B + (size_t)s.begin * ldb, ldb,
+            0.0, C + (size_t)s.begin * ldc, ldc, row, 0);
 }
 
 // (cut into slices of the columns like the others: see grouped_outer_kernel)
-__global__ __launch_bounds__(256, 2)
+template <bool FAST>
+__global__ __launch_bounds__(256, FAST ? 3 : 2)
 void grouped_douter_kernel(int groups, int m, int n, int k, int slices, int const *__restrict__ offsets, double const *__restrict__ X, int ldx,
     double const *__restrict__ Y, int ldy, double beta, double *__restrict__ D, int ldd, long strideD)
 {
@@ -325,15 +327,26 @@ void grouped_douter_kernel(int groups, int m, int n, int k, int slices, int cons
     int const length = s.end - s.begin, part = slices == 1 ? length : ((length + slices - 1) / slices + 15) / 16 * 16;
     int const begin = s.begin + (int)min((long)slice * part, (long)length), end = min(begin + part, s.end);
     double *const to = D + ((long)slice * groups + s.group) * strideD;
-    if (begin == end) {
+    if constexpr (FAST) {
+        __shared__ __attribute__((aligned(16))) char lds[DoubleTile<false, false>::LDS_BYTES];
+        int const r0 = row * 64, c0 = col * 64;
+        DoubleTile<false, false> one;
+        one.run(Plan<double>{X + (long)begin * ldx + r0, Y + (long)begin * ldy + c0, ldx, ldy, m - r0, n - c0, end - begin, 0, 0}, lds);
+        one.store(beta, to + (long)c0 * ldd + r0, ldd, m - r0, n - c0);
+    } else if (begin == end) {
         for (int e = threadIdx.x; e < 64 * 64; e += 256) {
             int const r = row * 64 + e % 64, c = col * 64 + e / 64;
             if (r < m && c < n) { double *const p = to + (size_t)c * ldd + r; *p = beta == 0.0 ? 0.0 : beta * *p; }
         }
-        return;
-    }
-    gemm_tile<64, 64, 16, false, true, 16>(m, n, end - begin, 1.0, X + (size_t)begin * ldx, ldx, Y + (size_t)begin * ldy, ldy,
-        beta, to, ldd, row, col);
+    } else
+        gemm_tile<64, 64, 16, false, true, 16>(m, n, end - begin, 1.0, X + (size_t)begin * ldx, ldx, Y + (size_t)begin * ldy, ldy,
+            beta, to, ldd, row, col);
+}
+
+// Whether an operand can be fed directly: columns aligned to 4 bytes, positions within a tile below 2^31 bytes (256 columns of up to 4 MB).
+static bool direct(void const *p, long ld, long stride, int size)
+{
+    return (uintptr_t)p % 4 == 0 && ld * size % 4 == 0 && stride * size % 4 == 0 && ld * size <= 1 << 22;
 }
 
 template <bool TA>
@@ -342,14 +355,9 @@ static hipError_t dgemm_launch(hipStream_t s, int groups, int m, int n, int k, i
 {
     long const tiles = most_pieces(groups, n, 64) * ((m + 63) / 64);
     if (tiles >= 1L << 31) return hipErrorInvalidConfiguration;
-    return launch_kernel(grouped_dgemm_kernel<TA>, dim3((unsigned)roundup(tiles, 8)), 256, s,
-        GemmCfg<64, 64, 16, TA, false>::LDS_BYTES, groups, m, n, k, offsets, A, lda, strideA, B, ldb, C, ldc);
-}
-
-// Whether an operand can be fed directly: columns aligned to 4 bytes, positions within a tile below 2^31 bytes (256 columns of up to 4 MB).
-static bool direct(void const *p, long ld, long stride, int size)
-{
-    return (uintptr_t)p % 4 == 0 && ld * size % 4 == 0 && stride * size % 4 == 0 && ld * size <= 1 << 22;
+    bool const fast = k == 0 || (direct(A, lda, strideA, 8) && direct(B, ldb, 0, 8));
+    return launch_kernel(fast ? grouped_dgemm_kernel<TA, true> : grouped_dgemm_kernel<TA, false>, dim3((unsigned)roundup(tiles, 8)), 256, s,
+        fast ? 0 : GemmCfg<64, 64, 16, TA, false>::LDS_BYTES, groups, m, n, k, offsets, A, lda, strideA, B, ldb, C, ldc);
 }
 
 // Workgroups for so many equal tiles: no more than the chip holds at once, each with a run of tiles, so that the loads of the next tile
@@ -506,7 +514,9 @@ hipError_t grouped_outer(hipStream_t s, ProductType type, ProductType typeD, int
         int const slices = work != nullptr && work_size >= grouped_outer_work_size(type, groups, m, n, k) ? douter_slices(groups, m, n, k) : 1;
         long const tiles = (long)groups * slices * ((m + 63) / 64) * ((n + 63) / 64);
         if (tiles >= 1L << 31) return hipErrorInvalidConfiguration;
-        hipError_t const e = launch_kernel(grouped_douter_kernel, dim3((unsigned)roundup(tiles, 8)), 256, s, GemmCfg<64, 64, 16, false, true>::LDS_BYTES,
+        bool const fast = direct(X, ldx, 0, 8) && direct(Y, ldy, 0, 8);
+        hipError_t const e = launch_kernel(fast ? grouped_douter_kernel<true> : grouped_douter_kernel<false>, dim3((unsigned)roundup(tiles, 8)), 256, s,
+            fast ? 0 : GemmCfg<64, 64, 16, false, true>::LDS_BYTES,
             groups, m, n, k, slices, offsets, (double const *)X, ldx, (double const *)Y, ldy, slices > 1 ? 0.0 : beta,
             slices > 1 ? (double *)work : (double *)D, slices > 1 ? m : ldd, slices > 1 ? (long)m * n : strideD);
         if (e != hipSuccess || slices == 1) return e;

@@ -691,3 +691,36 @@ def test_8_bit_groups_that_share_their_scales(node, tokens):
         torch.cuda.current_stream().cuda_stream) == 0
     sums = B.double() @ A[0].double().T.contiguous()
     assert torch.equal(C, scaled(sums, sa[0], sb, torch.float32))
+
+
+@pytest.mark.parametrize("trans", ["T", "N"])
+def test_f64_columns_too_far_apart_for_direct_loads(node, trans):
+    """Columns more than 4 MB apart are read by another kernel."""
+    import torch
+    gen, sizes, m, k, ld = generator(79), [3, 0, 5, 66], 70, 333, (1 << 19) + 3
+    n = sum(sizes)
+    far = torch.full((m + n + k + m, ld), float("nan"), dtype=torch.float64, device="cuda")
+    A = torch.randn(1, *((m, k) if trans == "T" else (k, m)), generator=gen, device="cuda", dtype=torch.float64)
+    B = torch.randn(n, k, generator=gen, device="cuda", dtype=torch.float64)
+    farA, farB = far[:A.shape[1], :A.shape[2]], far[m + k:m + k + n, :k]
+    farA.copy_(A[0]); farB.copy_(B)
+    near, there = torch.empty(n, m, dtype=torch.float64, device="cuda"), torch.empty(n, m, dtype=torch.float64, device="cuda")
+    off, groups = offsets_of(sizes), len(sizes)
+    assert node.grouped_gemm_device(trans, off, A.expand(groups, *A.shape[1:]), B, near) == 0
+    assert node.grouped_gemm_device(trans, off, farA[None].expand(groups, *A.shape[1:]), farB, there) == 0
+    a = A[0].T if trans == "T" else A[0]
+    ref = B @ a
+    bound = product_bound(k, B.abs() @ a.abs(), ref, torch.float64)
+    assert bool(((near - ref).abs() <= 2 * bound).all()) and bool(((there - ref).abs() <= 2 * bound).all())
+    # and without inner terms
+    assert node.grouped_gemm_device(trans, off, farA[None].expand(groups, *A.shape[1:])[:, :, :0] if trans == "T" else
+                                    farA[None].expand(groups, *A.shape[1:])[:, :0], farB[:, :0], there) == 0
+    assert bool((there == 0).all())
+    Y = torch.randn(n, 40, generator=gen, device="cuda", dtype=torch.float64)
+    for beta in (0.0, 0.5):
+        D = torch.ones(groups, 40, k, dtype=torch.float64, device="cuda")
+        E = D.clone()
+        assert node.grouped_outer_device(off, B, Y, D, beta=beta) == 0
+        assert node.grouped_outer_device(off, farB, Y, E, beta=beta) == 0
+        bound = product_bound(max(sizes) + 2, torch.stack([y.abs().T.contiguous() @ x.abs() for y, x in zip(Y.split(sizes), B.split(sizes))]) + beta, D, torch.float64)
+        assert bool(((D - E).abs() <= 2 * bound).all())
