@@ -103,17 +103,40 @@ void grouped_outer_kernel(int groups, int m, int n, int k, int slices, int const
     });
 }
 
-template <typename S, typename D>
+// PARTS threads an output, each with a run of the slices, eight of them in flight; the runs' sums in their order.  (1 thread with one load at a time: 64 planes of
+// 64 x 64 took 70 us, with 8 threads 5 us.)
+template <typename S, typename D, int PARTS>
 __global__ __launch_bounds__(256)
 void grouped_outer_sum_kernel(int groups, int m, int n, int slices, S const *__restrict__ planes, S beta, D *__restrict__ out, long ldd, long strideD)
 {
+    constexpr int WIDE = 256 / PARTS;
+    __shared__ S part[PARTS][WIDE];
     long const all = (long)groups * n * m;
-    for (long e = blockIdx.x * 256L + threadIdx.x; e < all; e += gridDim.x * 256L) {
-        S sum = planes[e];
-        for (int s = 1; s < slices; s++) sum += planes[s * all + e];
-        long const column = e / m;
-        D *const to = out + column / n * strideD + column % n * ldd + e % m;
-        *to = (D)(beta == 0 ? sum : sum + beta * (S)*to);
+    int const mine = threadIdx.x % WIDE, p = threadIdx.x / WIDE, each = (slices + PARTS - 1) / PARTS, end = min((p + 1) * each, slices);
+    for (long e0 = (long)blockIdx.x * WIDE; e0 < all; e0 += (long)gridDim.x * WIDE) {
+        long const e = e0 + mine;
+        S sum = 0;
+        if (e < all)
+            for (int s = p * each; s < end; s += 8) {
+                S v[8];
+                #pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = s + i < end ? planes[(s + i) * all + e] : (S)0;
+                #pragma unroll
+                for (int i = 0; i < 8; i++) sum += v[i];
+            }
+        if (PARTS > 1) {
+            part[p][mine] = sum;
+            __syncthreads();
+            if (p == 0)
+                #pragma unroll
+                for (int i = 1; i < PARTS; i++) sum += part[i][mine];
+            __syncthreads();
+        }
+        if (p == 0 && e < all) {
+            long const column = e / m;
+            D *const to = out + column / n * strideD + column % n * ldd + e % m;
+            *to = (D)(beta == 0 ? sum : sum + beta * (S)*to);
+        }
     }
 }
 
@@ -290,8 +313,8 @@ void grouped_gemm_few_kernel(int groups, int m, int n, int k, int const *__restr
 }
 
 // fp64: one piece of a group a workgroup; the tile rows of a piece side by side, so that its columns come from memory once.
-// FAST: operands that can be fed directly; others by the tile of the library's own dgemm.
 // (24 matrices 312 x 312, 40000 columns: 154 us, 51 TFLOP/s, with the tile of dgemm 172 us; 20000 columns, 8 matrices 1024 x 1024: 705 us, 60 TFLOP/s, 762 us)
+// FAST: operands that can be fed directly; others by the tile of the library's own dgemm.
 template <bool TA, bool FAST>
 __global__ __launch_bounds__(256, FAST ? 3 : 2)
 void grouped_dgemm_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, double const *__restrict__ A, int lda, long strideA,
@@ -311,6 +334,68 @@ void grouped_dgemm_kernel(int groups, int m, int n, int k, int const *__restrict
     } else          // (k > 0: this tile reads its operands' last inner term)
         gemm_tile<64, 64, 16, TA, false, 16>(m, s.end - s.begin, k, 1.0, A + s.group * strideA, lda, B + (size_t)s.begin * ldb, ldb,
             0.0, C + (size_t)s.begin * ldc, ldc, row, 0);
+}
+
+// fp64, too few 64 x 64 tiles to fill the chip: 16 x 16 outputs a workgroup, whose eight waves cut the inner index into eight runs, straight from memory; eight
+// steps of eight inner terms (8 s + 2 q + e for the lanes with q = lane >> 4, two instructions e) in flight.  Sums of 64 terms, added up in their turn.
+template <bool TA>
+__global__ __launch_bounds__(512)
+void grouped_dgemm_few_kernel(int groups, int m, int n, int k, int const *__restrict__ offsets, double const *__restrict__ A, long lda, long strideA,
+    double const *__restrict__ B, long ldb, double *__restrict__ C, long ldc)
+{
+    typedef double d2 __attribute__((ext_vector_type(2)));
+    typedef double d4 __attribute__((ext_vector_type(4)));
+    constexpr int WAVES = 8, U = 8;
+    __shared__ d4 sums[WAVES][64];
+    Pieces pieces(offsets, groups, n, 16);
+    int const t = tile_of_workgroup((m + 15) / 16 * pieces.total, 0);
+    if (t < 0) return;
+    Span const p = pieces.at((unsigned)t % (unsigned)pieces.total);
+    int const r0 = (unsigned)t / (unsigned)pieces.total * 16, rows = m - r0, cols = p.end - p.begin;
+    int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
+    int const steps = (k + 7) / 8, run = (steps + WAVES - 1) / WAVES, first = min(wave * run, steps), end = min(first + run, steps);
+    // (a row or column that is not there: another's, and its result is not stored)
+    double const *const a = A + p.group * strideA + (r0 + min(i, rows - 1)) * (TA ? lda : 1L), *const b = B + (p.begin + min(i, cols - 1)) * ldb;
+    d4 sum = {0.0, 0.0, 0.0, 0.0};
+    for (int s = first; s < end; s += U) {
+        d2 va[U], vb[U];
+        if (s + U <= min(end, k / 8)) {
+            #pragma unroll
+            for (int u = 0; u < U; u++) {
+                long const at = (s + u) * 8L + 2 * q;
+                if (TA) va[u] = __builtin_bit_cast(d2, load16(a + at));
+                else va[u] = d2{a[at * lda], a[(at + 1) * lda]};
+                vb[u] = __builtin_bit_cast(d2, load16(b + at));
+            }
+        } else {
+            #pragma unroll
+            for (int u = 0; u < U; u++)
+                #pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    int const at = (s + u) * 8 + 2 * q + e;
+                    long const from = min(at, k - 1);
+                    double const x = a[from * (TA ? 1L : lda)], y = b[from];
+                    bool const there = s + u < end && at < k;
+                    va[u][e] = there ? x : 0.0; vb[u][e] = there ? y : 0.0;
+                }
+        }
+        d4 acc = {0.0, 0.0, 0.0, 0.0};
+        #pragma unroll
+        for (int u = 0; u < U; u++)
+            #pragma unroll
+            for (int e = 0; e < 2; e++) acc = __builtin_amdgcn_mfma_f64_16x16x4f64(va[u][e], vb[u][e], acc, 0, 0, 0);
+        sum += acc;
+    }
+    sums[wave][lane] = sum;
+    __syncthreads();
+    // lane l, register r of a sum is row (l >> 4) + 4 r, column l & 15
+    if (threadIdx.x < 256) {
+        int const row = threadIdx.x & 15, col = threadIdx.x >> 4, l = (row & 3) * 16 + col;
+        double v = sums[0][l][row >> 2];
+        #pragma unroll
+        for (int w = 1; w < WAVES; w++) v += sums[w][l][row >> 2];
+        if (row < rows && col < cols) C[(p.begin + col) * ldc + r0 + row] = v;
+    }
 }
 
 // (cut into slices of the columns like the others: see grouped_outer_kernel)
@@ -355,6 +440,12 @@ static hipError_t dgemm_launch(hipStream_t s, int groups, int m, int n, int k, i
 {
     long const tiles = most_pieces(groups, n, 64) * ((m + 63) / 64);
     if (tiles >= 1L << 31) return hipErrorInvalidConfiguration;
+    // In us, fitted to 1 ... 640 columns, 426 ... 1152 rows and 300 ... 4096 inner terms.  1 column, 768 x 2624: 19 us (tiles of 64: 117 us); 64 columns, 512 x 512: 10 us
+    // (26 us); 576 columns, 512 x 4096: 143 us (180 us); 512 columns, 512 x 300: 21 us (17 us)
+    long const small = most_pieces(groups, n, 16) * ((m + 15) / 16);
+    if (k > 0 && 10 + 3.4e-5 * small * k < 6 + 0.0425 * k * std::max(1.0, tiles / 256.0) && small < 1L << 22)
+        return launch_kernel(grouped_dgemm_few_kernel<TA>, dim3((unsigned)roundup(small, 8)), 512, s, 0,
+            groups, m, n, k, offsets, A, (long)lda, strideA, B, (long)ldb, C, (long)ldc);
     bool const fast = k == 0 || (direct(A, lda, strideA, 8) && direct(B, ldb, 0, 8));
     return launch_kernel(fast ? grouped_dgemm_kernel<TA, true> : grouped_dgemm_kernel<TA, false>, dim3((unsigned)roundup(tiles, 8)), 256, s,
         fast ? 0 : GemmCfg<64, 64, 16, TA, false>::LDS_BYTES, groups, m, n, k, offsets, A, lda, strideA, B, ldb, C, ldc);
@@ -376,7 +467,7 @@ static unsigned resident(long tiles)
 //   tile 256: the fewest reads a product;                                   4096 columns, 4096 x 4096: 120 us (128: 143 us)
 static double tile_time(int tile, bool fast, double workgroups, double ktiles)
 {
-    double const w = std::max(1.0, workgroups), rounds = std::ceil(w / (tile == 128 ? 512 : 256) - 0.01);
+    double const w = std::max(1.0, workgroups), rounds = std::max(1.0, std::ceil(w / (tile == 128 ? 512 : 256) - 0.01));
     if (tile == 64) return rounds * ((fast ? 0.66 : 1.1) * std::ceil(ktiles / 4) + (fast ? 4.9 : 8.6));
     if (tile == 128) return w <= 256 ? (fast ? 0.62 : 0.9) * ktiles + 6 : rounds * ((fast ? 1.05 : 1.3) * ktiles + 6);
     return rounds * ((1.1 + 0.65 * std::min(1.0, w / 256)) * ktiles + 8);
@@ -467,6 +558,14 @@ static hipError_t outer_tiles(hipStream_t s, int slices, int groups, int m, int 
         groups, m, n, k, slices, offsets, (T const *)X, (long)ldx, (T const *)Y, (long)ldy, (float)beta, (D *)out, (long)ldd, strideD);
 }
 
+template <typename S, typename D>
+static hipError_t outer_sum(hipStream_t s, int slices, int groups, int m, int n, void const *work, double beta, void *out, int ldd, long strideD)
+{
+    int const wide = slices > 4 ? 32 : 256;
+    return launch_kernel(slices > 4 ? grouped_outer_sum_kernel<S, D, 8> : grouped_outer_sum_kernel<S, D, 1>,
+        dim3((unsigned)std::min(((long)groups * m * n + wide - 1) / wide, 16384L)), 256, s, 0, groups, m, n, slices, (S const *)work, (S)beta, (D *)out, (long)ldd, strideD);
+}
+
 template <typename T, typename D>
 static hipError_t outer_launch(hipStream_t s, int groups, int m, int n, int k, int const *offsets, void const *X, int ldx, void const *Y, int ldy,
     double beta, void *out, int ldd, long strideD, void *work, long work_size)
@@ -488,8 +587,7 @@ static hipError_t outer_launch(hipStream_t s, int groups, int m, int n, int k, i
     if (c.slices == 1) return go((D *)out, ldd, strideD, beta);
     hipError_t const e = go((float *)work, m, (long)m * n, 0.0);
     if (e != hipSuccess) return e;
-    return launch_kernel(grouped_outer_sum_kernel<float, D>, dim3((unsigned)std::min(((long)groups * m * n + 255) / 256, 4096L)), 256, s, 0,
-        groups, m, n, c.slices, (float const *)work, (float)beta, (D *)out, (long)ldd, strideD);
+    return outer_sum<float, D>(s, c.slices, groups, m, n, work, beta, out, ldd, strideD);
 }
 
 // fp64: as many slices as fill the chip's three workgroups a compute unit, of 256 columns at least
@@ -520,8 +618,7 @@ hipError_t grouped_outer(hipStream_t s, ProductType type, ProductType typeD, int
             groups, m, n, k, slices, offsets, (double const *)X, ldx, (double const *)Y, ldy, slices > 1 ? 0.0 : beta,
             slices > 1 ? (double *)work : (double *)D, slices > 1 ? m : ldd, slices > 1 ? (long)m * n : strideD);
         if (e != hipSuccess || slices == 1) return e;
-        return launch_kernel(grouped_outer_sum_kernel<double, double>, dim3((unsigned)std::min(((long)groups * m * n + 255) / 256, 4096L)), 256, s, 0,
-            groups, m, n, slices, (double const *)work, beta, (double *)D, (long)ldd, strideD);
+        return outer_sum<double, double>(s, slices, groups, m, n, work, beta, D, ldd, strideD);
     }
     bool const wide = typeD == PRODUCT_F32;
     auto const launch = type == PRODUCT_BF16 ? (wide ? outer_launch<__bf16, float> : outer_launch<__bf16, __bf16>)

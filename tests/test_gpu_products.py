@@ -697,12 +697,13 @@ def test_8_bit_groups_that_share_their_scales(node, tokens):
 def test_f64_columns_too_far_apart_for_direct_loads(node, trans):
     """Columns more than 4 MB apart are read by another kernel."""
     import torch
-    gen, sizes, m, k, ld = generator(79), [3, 0, 5, 66], 70, 333, (1 << 19) + 3
+    gen, sizes, m, k, ld = generator(79), [300, 0, 500, 266], 330, 333, (1 << 19) + 3
     n = sum(sizes)
-    far = torch.full((m + n + k + m, ld), float("nan"), dtype=torch.float64, device="cuda")
+    far = torch.empty((n + 340, ld), dtype=torch.float64, device="cuda")
+    far[:, :400] = float("nan")
     A = torch.randn(1, *((m, k) if trans == "T" else (k, m)), generator=gen, device="cuda", dtype=torch.float64)
     B = torch.randn(n, k, generator=gen, device="cuda", dtype=torch.float64)
-    farA, farB = far[:A.shape[1], :A.shape[2]], far[m + k:m + k + n, :k]
+    farA, farB = far[:A.shape[1], :A.shape[2]], far[340:, :k]
     farA.copy_(A[0]); farB.copy_(B)
     near, there = torch.empty(n, m, dtype=torch.float64, device="cuda"), torch.empty(n, m, dtype=torch.float64, device="cuda")
     off, groups = offsets_of(sizes), len(sizes)
@@ -724,3 +725,27 @@ def test_f64_columns_too_far_apart_for_direct_loads(node, trans):
         assert node.grouped_outer_device(off, farB, Y, E, beta=beta) == 0
         bound = product_bound(max(sizes) + 2, torch.stack([y.abs().T.contiguous() @ x.abs() for y, x in zip(Y.split(sizes), B.split(sizes))]) + beta, D, torch.float64)
         assert bool(((D - E).abs() <= 2 * bound).all())
+
+
+@pytest.mark.parametrize("trans", ["T", "N"])
+@pytest.mark.parametrize("k", [1, 2, 3, 15, 16, 17, 31, 33, 48, 257, 300])
+@pytest.mark.parametrize("pads,shifts", [((0, 0, 0), (0, 0, 0)), ((1, 3, 5), (1, 0, 3))])
+def test_f64_tiles(node, trans, k, pads, shifts):
+    """Enough tiles for those of 64 x 64, inner lengths around theirs of 16."""
+    check_product(node, trans, "f64", [300, 0, 450, 1, 64], 701, k, first=2, behind=3, pads=pads, shifts=shifts, seed=83)
+
+
+@pytest.mark.parametrize("trans", ["T", "N"])
+@pytest.mark.parametrize("k", [1, 7, 8, 9, 63, 64, 65, 500, 519])
+@pytest.mark.parametrize("pads,shifts", [((0, 0, 0), (0, 0, 0)), ((1, 3, 5), (1, 0, 3))])
+def test_f64_of_few_columns(node, trans, k, pads, shifts):
+    """Few outputs: 16 columns a workgroup, whose waves cut inner lengths around multiples of 8 and 64."""
+    check_product(node, trans, "f64", [3, 0, 17, 40], 50, k, first=2, behind=3, pads=pads, shifts=shifts, seed=89)
+
+
+@pytest.mark.parametrize("type_,out", [("bf16", "f32"), ("f16", "f16"), ("f64", "f64")])
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+@pytest.mark.parametrize("k,m,n", [(4203, 64, 64), (2118, 70, 9), (9000, 33, 130), (700, 64, 64)])
+def test_outer_of_long_sums(node, type_, out, beta, k, m, n):
+    """Few outputs, many slices, whose sums several threads add up."""
+    check_outer(node, type_, out, [k], m, n, beta, pads=(0, 2, 1), shifts=(0, 0, 0), seed=97)
