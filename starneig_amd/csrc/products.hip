@@ -104,7 +104,7 @@ void grouped_outer_kernel(int groups, int m, int n, int k, int slices, int const
 }
 
 // PARTS threads an output, each with a run of the slices, eight of them in flight; the runs' sums in their order.  (1 thread with one load at a time: 64 planes of
-// 64 x 64 took 70 us, with 8 threads 5 us.)
+// 64 x 64 in fp64 took 18 us, with 8 threads 3.9 us; 4 planes of 512 x 512 in fp32 take 3.9 us either way.)
 template <typename S, typename D, int PARTS>
 __global__ __launch_bounds__(256)
 void grouped_outer_sum_kernel(int groups, int m, int n, int slices, S const *__restrict__ planes, S beta, D *__restrict__ out, long ldd, long strideD)
