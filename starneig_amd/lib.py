@@ -513,14 +513,24 @@ def dgemm_device(transA, transB, m, n, k, alpha, tA, ldA, tB, ldB, beta, tC, ldC
 AMD_F64, AMD_F32, AMD_BF16, AMD_F16 = range(4)
 
 
-_product_types = {}
+_product_torch = None
+
+
+def _product_setup():
+    """(codes of the types, the types int32, int8 and float32, functions for the current device and for a device's current stream)."""
+    global _product_torch
+    import torch
+    # (the unwrapped functions: torch.cuda.current_stream() alone takes a third of a small call's time)
+    _product_torch = (
+        {torch.float64: AMD_F64, torch.float32: AMD_F32, torch.bfloat16: AMD_BF16, torch.float16: AMD_F16},
+        torch.int32, torch.int8, torch.float32,
+        getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
+        getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: _stream_ptr()))
+    return _product_torch
 
 
 def _product_type(t):
-    if not _product_types:
-        import torch
-        _product_types.update({torch.float64: AMD_F64, torch.float32: AMD_F32, torch.bfloat16: AMD_BF16, torch.float16: AMD_F16})
-    code = _product_types.get(t.dtype)
+    code = _product_torch[0].get(t.dtype)
     if code is None:
         raise ValueError(f"no product takes {t.dtype}")
     return code
@@ -528,13 +538,11 @@ def _product_type(t):
 
 def _product_device(t):
     """(device, its current stream) of a call whose tensors have to be on the current device."""
-    import torch
     device = t.get_device()
-    if device < 0 or device != torch.cuda.current_device():
+    torch = _product_torch or _product_setup()
+    if device < 0 or device != torch[4]():
         raise ValueError(f"a tensor is on {t.device}, not on the current device")
-    # (a fortieth of the time of torch.cuda.current_stream(), which is a third of a small call's)
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return device, raw(device) if raw else _stream_ptr()
+    return device, torch[5](device)
 
 
 def _product_matrix(name, t, shape, dtype, device):
@@ -546,41 +554,42 @@ def _product_matrix(name, t, shape, dtype, device):
     if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, not on the current device")
     rows, stride = shape[-1], t.stride()
+    dims = len(stride)
     if stride[-1] != 1 and rows > 1 and t.numel():
         raise ValueError(f"the last dimension of {name} is not contiguous")
-    dims = len(stride)
     if dims == 1:
         return t.data_ptr(), rows, 0
     # (the stride of a dimension of one entry says nothing)
-    ld = stride[-2] if shape[-2] > 1 else max(1, rows)
+    ld = stride[-2] if shape[-2] > 1 else rows or 1
     if ld < rows or ld > 0x7fffffff:
         raise ValueError(f"the columns of {name} overlap or lie 2^31 entries apart")
     return t.data_ptr(), ld, (stride[0] if dims == 3 and shape[0] > 1 else 0)
 
 
 def _product_sizes(name, t):
-    if t.dim() != 2:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not (columns, rows)")
-    if t.shape[0] > 0x7fffffff:
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} has shape {tuple(shape)}, not (columns, rows)")
+    if shape[0] > 0x7fffffff:
         raise ValueError(f"{name} has 2^31 columns or more")
-    return t.shape
+    return shape
 
 
 def _product_offsets(t, device):
     """(pointer, groups) of the groups' first columns, int32, the end of the last group behind them."""
-    import torch
-    if t.dim() != 1 or t.shape[0] < 2:
+    shape = t.shape
+    if len(shape) != 1 or shape[0] < 2:
         raise ValueError("offsets hold one number more than there are groups, of which there is at least one")
-    return _product_matrix("offsets", t, t.shape, torch.int32, device)[0], t.shape[0] - 1
+    return _product_matrix("offsets", t, shape, _product_torch[1], device)[0], shape[0] - 1
 
 
 def grouped_gemm_device(transA, tOffsets, tA, tB, tC):
     """C_g = op(A_g) B_g: tB (n, k), tC (n, m), tA (groups, m, k) for "T", (groups, k, m) for "N"."""
     (device, stream), dtype = _product_device(tB), tB.dtype
     poff, groups = _product_offsets(tOffsets, device)
-    n, k = _product_sizes("B", tB)
+    n, k = shape = _product_sizes("B", tB)
     m = _product_sizes("C", tC)[1]
-    pb, ldb, _ = _product_matrix("B", tB, (n, k), dtype, device)
+    pb, ldb, _ = _product_matrix("B", tB, shape, dtype, device)
     pc, ldc, _ = _product_matrix("C", tC, (n, m), dtype, device)
     pa, lda, stride = _product_matrix("A", tA, (groups, m, k) if transA in ("T", "t") else (groups, k, m), dtype, device)
     return load().starneig_amd_grouped_gemm_device(
@@ -609,22 +618,22 @@ def grouped_outer_device(tOffsets, tX, tY, tD, beta=0.0):
 
 def quantize_i8_device(tX, tQ, tScale):
     """tQ (n, k) int8 and tScale (n) float32 of tX (n, k): Q = rint(X / scale), scale = max |X| / 127 of the column."""
-    import torch
     device, stream = _product_device(tX)
-    n, k = _product_sizes("X", tX)
-    px, ldx, _ = _product_matrix("X", tX, (n, k), tX.dtype, device)
-    pq, ldq, _ = _product_matrix("Q", tQ, (n, k), torch.int8, device)
-    ps, _, _ = _product_matrix("scale", tScale, (n,), torch.float32, device)
+    _, _, i8, f32, _, _ = _product_torch
+    n, k = shape = _product_sizes("X", tX)
+    px, ldx, _ = _product_matrix("X", tX, shape, tX.dtype, device)
+    pq, ldq, _ = _product_matrix("Q", tQ, shape, i8, device)
+    ps, _, _ = _product_matrix("scale", tScale, (n,), f32, device)
     return load().starneig_amd_quantize_i8_device(_product_type(tX), k, n, px, ldx, pq, ldq, ps, stream)
 
 
 def gemm_i8_device(tA, tScaleA, tB, tScaleB, tC):
     """C = (A^T B) scaled by row and column: tA (m, k) and tB (n, k) int8, tScaleA (m) and tScaleB (n) float32, tC (n, m)."""
-    import torch
-    (device, stream), i8, f32 = _product_device(tB), torch.int8, torch.float32
-    n, k = _product_sizes("B", tB)
+    device, stream = _product_device(tB)
+    _, _, i8, f32, _, _ = _product_torch
+    n, k = shape = _product_sizes("B", tB)
     m = _product_sizes("C", tC)[1]
-    pb, ldb, _ = _product_matrix("B", tB, (n, k), i8, device)
+    pb, ldb, _ = _product_matrix("B", tB, shape, i8, device)
     pc, ldc, _ = _product_matrix("C", tC, (n, m), tC.dtype, device)
     pa, lda, _ = _product_matrix("A", tA, (m, k), i8, device)
     psa, _, _ = _product_matrix("scaleA", tScaleA, (m,), f32, device)
@@ -634,12 +643,12 @@ def gemm_i8_device(tA, tScaleA, tB, tScaleB, tC):
 
 def grouped_gemm_i8_device(tOffsets, tA, tScaleA, tB, tScaleB, tC):
     """The same with tA (groups, m, k) and tScaleA (groups, m) for the columns of every group."""
-    import torch
-    (device, stream), i8, f32 = _product_device(tB), torch.int8, torch.float32
+    device, stream = _product_device(tB)
+    _, _, i8, f32, _, _ = _product_torch
     poff, groups = _product_offsets(tOffsets, device)
-    n, k = _product_sizes("B", tB)
+    n, k = shape = _product_sizes("B", tB)
     m = _product_sizes("C", tC)[1]
-    pb, ldb, _ = _product_matrix("B", tB, (n, k), i8, device)
+    pb, ldb, _ = _product_matrix("B", tB, shape, i8, device)
     pc, ldc, _ = _product_matrix("C", tC, (n, m), tC.dtype, device)
     pa, lda, stride = _product_matrix("A", tA, (groups, m, k), i8, device)
     psa, ldsa, _ = _product_matrix("scaleA", tScaleA, (groups, m), f32, device)
