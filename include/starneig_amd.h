@@ -153,7 +153,8 @@ starneig_error_t starneig_amd_dgemm_device(
  * on several streams at once and be captured into graphs.  All pointers are on the current device and aligned to their
  * elements; outputs must not overlap inputs; m, n and k are at most 2^30, groups
  * 65535.  Columns aligned to 4 bytes (pointer, leading dimension, stride) are read fastest.
- * fp16 / bf16 sums are held in fp32 and rounded once, fp64 sums as in starneig_amd_dgemm_device; equal calls give
+ * fp16 / bf16 sums are held in fp32 and rounded once, fp64 sums are taken in parts of at most 256 terms
+ * like those of starneig_amd_dgemm_device; equal calls give
  * equal bits.  A return value of -i marks the i-th argument, STARNEIG_GENERIC_ERROR a launch that failed (sizes beyond
  * 2^32 threads included). */
 enum starneig_amd_type { STARNEIG_AMD_F64 = 0, STARNEIG_AMD_F32 = 1, STARNEIG_AMD_BF16 = 2, STARNEIG_AMD_F16 = 3 };
