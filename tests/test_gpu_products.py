@@ -749,3 +749,11 @@ def test_f64_of_few_columns(node, trans, k, pads, shifts):
 def test_outer_of_long_sums(node, type_, out, beta, k, m, n):
     """Few outputs, many slices, whose sums several threads add up."""
     check_outer(node, type_, out, [k], m, n, beta, pads=(0, 2, 1), shifts=(0, 0, 0), seed=97)
+
+
+@pytest.mark.parametrize("trans", ["T", "N"])
+@pytest.mark.parametrize("k", [1, 17, 32, 63, 270])
+@pytest.mark.parametrize("pads,shifts", [((0, 0, 0), (0, 0, 0)), ((1, 3, 5), (1, 0, 3))])
+def test_f64_of_many_tiles(node, trans, k, pads, shifts):
+    """More tiles than the chip holds at once."""
+    check_product(node, trans, "f64", [3000, 0, 1, 700], 701, k, first=2, behind=3, pads=pads, shifts=shifts, seed=101)
