@@ -54,14 +54,14 @@ struct Operand {
     static constexpr int CR = ROWS / EL;                    // MN: chunks a row
 
     // (ds_read_b128 serves 16 lanes at a time: 0-3, 12-15, 20-27; 4-11, 16-19, 28-31; and so on; ds_read_b64_tr_b16 32)
-    static __device__ __forceinline__ int swizzle_k(int r) { return sizeof(T) == 8 ? r >> 1 & 7 : (r >> 1 & 1) | (r >> 3 & 6); }
-    static __device__ __forceinline__ int swizzle_mn(int k) { return sizeof(T) == 8 ? 0 : CR >= 16 ? (k & 3) << 2 : (k & 2) << 1; }
+    static __host__ __device__ __forceinline__ int swizzle_k(int r) { return sizeof(T) == 8 ? r >> 1 & 7 : (r >> 1 & 1) | (r >> 3 & 6); }
+    static __host__ __device__ __forceinline__ int swizzle_mn(int k) { return sizeof(T) == 8 ? 0 : CR >= 16 ? (k & 3) << 2 : (k & 2) << 1; }
 
     // row of lane i of fragment t of 64 rows
     static __device__ __forceinline__ int row(int i, int t) { return K ? 8 * (i >> 2) + 4 * t + (i & 3) : 32 * t + i; }
 
     // outer and inner position, inside the tile, of the chunk that goes to place e
-    static __device__ __forceinline__ void chunk(int e, int &outer, int &inner)
+    static __host__ __device__ __forceinline__ void chunk(int e, int &outer, int &inner)
     {
         if (K) { outer = e >> 3; inner = ((e & 7) ^ swizzle_k(outer)) * EL; }
         else   { inner = e / CR; outer = ((e % CR) ^ swizzle_mn(inner)) * EL; }
@@ -131,39 +131,54 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
     T const *base;
     long step;                      // MN: numbers between k-tiles
     int k, ld, outers;
-    unsigned at[O::LOADS];          // byte offsets of the thread's chunks; beyond the buffer where there is nothing to read
+    unsigned at[O::LOADS];          // byte offsets of the thread's chunks
+
+    // Which bytes a k-tile's loads read; the tests compute them on the host.  Offsets from 2^31 on read zeros.
+    static constexpr unsigned NOTHING = 0x80000000u;
+    // Where chunk e of a tile lies: nowhere if it is past the outer end.
+    static __host__ __device__ __forceinline__ unsigned offset(int e, int outers, int ld)
+    {
+        int outer, inner;
+        O::chunk(e, outer, inner);
+        return outer < outers ? (unsigned)(((K ? outer : inner) * ld + (K ? inner : outer)) * (int)sizeof(T)) : NOTHING;
+    }
+    // Whether chunk e lies behind the `left` inner terms that there are from this k-tile's first on.
+    static __host__ __device__ __forceinline__ bool behind(int e, int left)
+    {
+        int outer, inner;
+        O::chunk(e, outer, inner);
+        return inner >= left;
+    }
+    // The bytes of the buffer: up to the last word of the operand (words, four bytes: the hardware tests each), where a chunk may reach it.  In the
+    // last k-tile that is a chunk that starts in front of the end; MN, where a chunk is wider than the leading dimension, also one of the rows in front
+    // of them, which covers the next rows' numbers: up to EL rows.  Behind the last k-tile the buffer is empty.
+    static __host__ __device__ __forceinline__ int bytes(int left, int outers, int ld)
+    {
+        if (left <= 0) return 0;
+        if (left > (K ? O::KT : O::KT + O::EL)) return 0x7fffffff;
+        int const rows = outers < ROWS ? outers : ROWS, wide = outers < ROWS + O::EL ? outers : ROWS + O::EL;
+        return (K ? (rows - 1) * ld + left : (left - 1) * ld + wide) * (int)sizeof(T) + 3 & ~3;
+    }
 
     __device__ __forceinline__ void set(T const *base_, int outers_, int k_, long ld_)
     {
         base = base_; k = k_; ld = (int)ld_; outers = outers_; step = ld_ * O::KT;
         int const thread = thread_now() % THREADS;
         #pragma unroll
-        for (int s = 0; s < O::LOADS; s++) {
-            int outer, in;
-            O::chunk(s * THREADS + thread, outer, in);
-            int const far = K ? outer : in, near = K ? in : outer;
-            at[s] = outer < outers ? (unsigned)((far * ld + near) * (int)sizeof(T)) : 0x80000000u;
-        }
+        for (int s = 0; s < O::LOADS; s++) at[s] = offset(s * THREADS + thread, outers, ld);
     }
-    // Loads 0 ... LOADS - 1 of k-tile kt to `lds`, after begin(kt); k-tiles are fetched in order.  Offsets from 2^31 on read zeros: positions past the
-    // outer end, and, in the last k-tile, the chunks past k.  So do the words past the operand's end there, with which a chunk that starts in front of
-    // it may end.  (Words, four bytes: the hardware tests each.)  Behind the last k-tile the buffer is empty.
+    // Loads 0 ... LOADS - 1 of k-tile kt to `lds`, after begin(kt); k-tiles are fetched in order.
     i32x4 from;
     __device__ __forceinline__ void begin(int kt)
     {
         int const left = k - kt * O::KT;
-        int bytes = left > 0 ? 0x7fffffff : 0;
         if (left <= O::KT && left > 0) {
             int const thread = thread_now() % THREADS;
             #pragma unroll
-            for (int s = 0; s < O::LOADS; s++) {
-                int outer, inner;
-                O::chunk(s * THREADS + thread, outer, inner);
-                if (inner >= left) at[s] = 0x80000000u;
-            }
-            bytes = (K ? (min(outers, ROWS) - 1) * ld + left : (left - 1) * ld + min(outers, ROWS + O::EL)) * (int)sizeof(T) + 3 & ~3;
+            for (int s = 0; s < O::LOADS; s++)
+                if (behind(s * THREADS + thread, left)) at[s] = NOTHING;
         }
-        from = buffer(K ? base + (long)kt * O::KT : base + kt * step, bytes);
+        from = buffer(K ? base + (long)kt * O::KT : base + kt * step, bytes(left, outers, ld));
     }
     __device__ __forceinline__ void load(int lds, int s) const { load_to_lds(from, at[s], lds + wave_number() % (THREADS / 64) * 1024 + s * THREADS * 16); }
     __device__ __forceinline__ void fetch(int lds, int kt)

@@ -821,3 +821,46 @@ hipError_t quantize_i8(hipStream_t s, ProductType type, int k, int n, void const
 }
 
 } // namespace sn
+
+#ifdef SN_TEST_HOOKS   // compiled into libstarneig_amd_test.so only (csrc/Makefile), never into the product library
+namespace {
+// The bytes that the direct loads of an operand read past its last word, at most over all k-tiles (0: none).  Every word of a chunk is
+// read whose four bytes lie in front of the buffer's end.
+template <typename T, int ROWS, bool K>
+long reads_past(int outers, int k, int ld)
+{
+    using S = sn::Stream<T, ROWS, K, 256, sn::DIRECT>;
+    using O = typename S::O;
+    long const end = ((K ? (long)(outers - 1) * ld + k : (long)(k - 1) * ld + outers) * (long)sizeof(T) + 3) / 4 * 4;
+    long past = 0;
+    for (int kt = 0; kt < (k + O::KT - 1) / O::KT + 2; kt++) {
+        int const left = k - kt * O::KT;
+        unsigned const bytes = (unsigned)S::bytes(left, outers, ld);
+        long const base = (K ? (long)kt * O::KT : (long)kt * O::KT * ld) * (long)sizeof(T);
+        for (int e = 0; e < ROWS * 8; e++) {
+            if (left <= O::KT && left > 0 && S::behind(e, left)) continue;
+            for (int w = 0; w < 4; w++) {
+                unsigned long const at = (unsigned long)S::offset(e, outers, ld) + 4 * w;
+                if (at + 4 <= bytes && base + (long)at + 4 - end > past) past = base + (long)at + 4 - end;
+            }
+        }
+    }
+    return past;
+}
+template <typename T>
+long reads_past(int tile, bool inner_contiguous, int outers, int k, int ld)
+{
+    auto const f = tile == 64 ? inner_contiguous ? reads_past<T, 64, true> : reads_past<T, 64, false>
+        : tile == 128 ? inner_contiguous ? reads_past<T, 128, true> : reads_past<T, 128, false>
+        : inner_contiguous ? reads_past<T, 256, true> : reads_past<T, 256, false>;
+    return f(outers, k, ld);
+}
+}
+// size: bytes of a number
+extern "C" __attribute__((visibility("default")))
+long sn_internal_product_reads_past(int size, int tile, int inner_contiguous, int outers, int k, int ld)
+{
+    return size == 1 ? reads_past<signed char>(tile, true, outers, k, ld) : size == 2 ? reads_past<__bf16>(tile, inner_contiguous, outers, k, ld)
+        : inner_contiguous ? reads_past<double, 64, true>(outers, k, ld) : reads_past<double, 64, false>(outers, k, ld);
+}
+#endif  // SN_TEST_HOOKS
