@@ -9,6 +9,12 @@
 
 namespace sn {
 
+#ifdef SN_TEST_HOOKS
+static int forced_tile = 0, forced_slices = 0;         // a test's choice in place of the rules' (0: theirs)
+#else
+static constexpr int forced_tile = 0, forced_slices = 0;
+#endif
+
 // a tile's place in the matrices
 struct Place { Span s; bool there; };
 
@@ -443,7 +449,7 @@ static hipError_t dgemm_launch(hipStream_t s, int groups, int m, int n, int k, i
     // In us, fitted to 1 ... 640 columns, 426 ... 1152 rows and 300 ... 4096 inner terms.  1 column, 768 x 2624: 19 us (tiles of 64: 117 us); 64 columns, 512 x 512: 10 us
     // (26 us); 576 columns, 512 x 4096: 143 us (180 us); 512 columns, 512 x 300: 21 us (17 us)
     long const small = most_pieces(groups, n, 16) * ((m + 15) / 16);
-    if (k > 0 && 10 + 3.4e-5 * small * k < 6 + 0.0425 * k * std::max(1.0, tiles / 256.0) && small < 1L << 22)
+    if (k > 0 && !forced_tile && 10 + 3.4e-5 * small * k < 6 + 0.0425 * k * std::max(1.0, tiles / 256.0) && small < 1L << 22)
         return launch_kernel(grouped_dgemm_few_kernel<TA>, dim3((unsigned)roundup(small, 8)), 512, s, 0,
             groups, m, n, k, offsets, A, (long)lda, strideA, B, (long)ldb, C, (long)ldc);
     bool const fast = k == 0 || (direct(A, lda, strideA, 8) && direct(B, ldb, 0, 8));
@@ -475,6 +481,7 @@ static double tile_time(int tile, bool fast, double workgroups, double ktiles)
 // The tile of a product.  The host does not know the groups' lengths: it counts the pieces that exponentially distributed ones of this mean have.
 static int product_tile(bool fast, int groups, int m, int n, int ktiles)
 {
+    if (forced_tile) return forced_tile;
     int best = 64;
     double least = 0;
     for (int tile : {64, 128, 256}) {
@@ -489,7 +496,7 @@ static int product_tile(bool fast, int groups, int m, int n, int ktiles)
 }
 // Few columns a group on average, and too few 64 x 64 tiles to fill the chip: 16 columns, 4096 x 4096: 11 us, in tiles of 64 15 us; 256 columns of 32
 // groups, 2048 x 1408: 62 us, in tiles of 128 32 us.
-static bool few_columns(int groups, int m, int n) { return (long)n <= 16L * groups && most_pieces(groups, n, 64) * ((m + 63) / 64) < 256; }
+static bool few_columns(int groups, int m, int n) { return !forced_tile && (long)n <= 16L * groups && most_pieces(groups, n, 64) * ((m + 63) / 64) < 256; }
 
 template <typename T, typename P>
 static hipError_t gemm_tiles(hipStream_t s, int groups, int m, int n, int k, int const *offsets, void const *A, int lda, long strideA,
@@ -539,6 +546,7 @@ static double outer_time(Cut c, bool fast, long groups, long m, long n, long k)
 static Cut outer_cut(bool fast, long groups, long m, long n, long k)
 {
     Cut best = {128, 1};
+    if (forced_tile) return Cut{forced_tile, forced_slices};
     for (int tile : {256, 128, 64})
         for (int slices : {1, 2, 4, 8, 16, 32, 64}) {
             Cut const c = {tile, slices};
@@ -593,6 +601,7 @@ static hipError_t outer_launch(hipStream_t s, int groups, int m, int n, int k, i
 // fp64: as many slices as fill the chip's three workgroups a compute unit, of 256 columns at least
 static int douter_slices(long groups, long m, long n, long k)
 {
+    if (forced_tile) return forced_slices;
     long const tiles = groups * ((m + 63) / 64) * ((n + 63) / 64);
     return (int)std::max(1L, std::min({768 / tiles, k / groups / 256, 64L}));
 }
@@ -863,4 +872,8 @@ long sn_internal_product_reads_past(int size, int tile, int inner_contiguous, in
     return size == 1 ? reads_past<signed char>(tile, true, outers, k, ld) : size == 2 ? reads_past<__bf16>(tile, inner_contiguous, outers, k, ld)
         : inner_contiguous ? reads_past<double, 64, true>(outers, k, ld) : reads_past<double, 64, false>(outers, k, ld);
 }
+// From here on products by tiles of this size (64, 128, 256 where columns are aligned), sums over columns in this many slices (at least 1);
+// 0: as the rules have it.
+extern "C" __attribute__((visibility("default")))
+void sn_internal_product_force(int tile, int slices) { sn::forced_tile = tile; sn::forced_slices = slices; }
 #endif  // SN_TEST_HOOKS

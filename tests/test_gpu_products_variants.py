@@ -1,0 +1,129 @@
+"""GPU: every variant of the products' tiles, whatever the rules that choose among them: tile, feed and slices are forced through the
+test-support library, with several tiles a workgroup, inner lengths that cut a chunk in the first, a middle and the last k-tile, and
+sums that are added to what is there.  Bounds as in test_gpu_products.py."""
+import pytest
+
+from helpers import U
+from test_gpu_products import check_outer, check_product, generator, kind, offsets_of, scaled, whole
+
+pytestmark = pytest.mark.gpu
+
+# more tiles of every size than workgroups fit the chip: 1000 tiles of 128 x 128, 300 of 256 x 256 with 2056 rows
+MANY = [1000, 0, 3000, 2100, 77, 2500]
+DIRECT, STAGED = ((0, 0, 0), (0, 0, 0)), ((1, 3, 5), (1, 0, 3))
+
+
+@pytest.fixture(scope="module")
+def library(node):
+    lib = node.lib.load_test_hooks()
+    for name, (res, args) in node.lib.SIGNATURES.items():
+        f = getattr(lib, name)
+        f.restype, f.argtypes = res, args
+    lib.starneig_node_init(1, 1, node.NO_MESSAGES)
+    yield lib
+    lib.starneig_node_finalize()
+
+
+@pytest.fixture
+def forced(node, library, monkeypatch):
+    """force(tile, slices): the binding's products run in the test-support library with this choice."""
+    monkeypatch.setattr(node.lib, "_lib", library)
+
+    def force(tile, slices=1):
+        library.sn_internal_product_force(tile, slices)
+    yield force
+    library.sn_internal_product_force(0, 0)
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f16"])
+@pytest.mark.parametrize("trans", ["T", "N"])
+@pytest.mark.parametrize("tile,feed", [(64, DIRECT), (128, DIRECT), (256, DIRECT), (64, STAGED), (128, STAGED)])
+@pytest.mark.parametrize("k", [42, 168, 301])
+def test_product(node, forced, trans, type_, tile, feed, k):
+    forced(tile)
+    aligned = feed == DIRECT
+    # (aligned columns: even leading dimensions)
+    pads, shifts = ((k % 2 if trans == "T" else 0, k % 2, 0), feed[1]) if aligned else feed
+    check_product(node, trans, type_, MANY, 2056 + 2 * aligned, k, first=2, behind=3, pads=pads, shifts=shifts)
+    check_product(node, trans, type_, [3, 0, 17, 1], 34, k, first=2, behind=3, pads=pads, shifts=shifts)
+
+
+@pytest.mark.parametrize("trans", ["T", "N"])
+@pytest.mark.parametrize("tile", [64, 128, 256])
+@pytest.mark.parametrize("m", [1, 2, 3, 4])
+def test_product_of_hardly_any_rows(node, forced, trans, tile, m):
+    """Leading dimensions smaller than a chunk, inner lengths just past a k-tile."""
+    forced(tile)
+    for k in (63, 64, 65, 66, 67, 129, 130):
+        check_product(node, trans, "bf16", [5, 0, 70], m, k, pads=(k % 2 if trans == "T" else m % 2, k % 2, 0))
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("tile,pad,shift", [(64, 0, 0), (128, 0, 0), (256, 0, 0), (64, 3, 5), (128, 3, 5)])
+@pytest.mark.parametrize("k", [42, 333, 400])
+def test_8_bit_product(node, forced, out, tile, pad, shift, k):
+    import torch
+    forced(tile)
+    pad = pad if shift else -k % 4
+    for sizes, m in ((MANY, 2058), ([3, 0, 17, 1], 34)):
+        gen, groups, first, behind = generator(k), len(sizes), 2, 3
+        n = first + sum(sizes) + behind
+        A, B = whole(gen, groups, m, k, pad=pad, shift=shift), whole(gen, n, k, pad=pad, shift=shift)
+        sa, sb = torch.rand(groups, m, generator=gen, device="cuda") * 1e-2, torch.rand(n, generator=gen, device="cuda") * 1e-2
+        C = torch.full((n, m + 3), 7.0, dtype=kind(out), device="cuda")
+        assert node.grouped_gemm_i8_device(offsets_of(sizes, first), A, sa, B, sb, C[:, :m]) == 0
+        at = first
+        for g, s in enumerate(sizes):
+            sums = B[at:at + s].double() @ A[g].double().T.contiguous()
+            assert torch.equal(C[at:at + s, :m], scaled(sums, sa[g], sb[at:at + s], kind(out))), g
+            at += s
+        assert bool((C[:, m:] == 7.0).all()) and bool((C[:first] == 7.0).all()) and bool((C[n - behind:] == 7.0).all())
+
+
+@pytest.mark.parametrize("type_,out", [("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+@pytest.mark.parametrize("slices", [1, 2, 7, 64])
+@pytest.mark.parametrize("tile,feed", [(64, DIRECT), (128, DIRECT), (256, DIRECT), (64, STAGED), (128, STAGED)])
+def test_outer(node, forced, type_, out, beta, slices, tile, feed):
+    forced(tile, slices)
+    pads, shifts = ((0, 0, 3), feed[1]) if feed == DIRECT else feed
+    check_outer(node, type_, out, [300, 0, 1000, 65, 5, 777, 128, 1], 1096, 1544, beta, first=2, behind=3, pads=pads, shifts=shifts)
+    # more groups than a wave has lanes; rows and columns of less than a chunk (aligned), of just one (not)
+    check_outer(node, type_, out, [1] * 40 + [65, 0, 66, 130] * 8, 10, 8 + 2 * (feed == DIRECT), beta, first=1, behind=1, pads=pads, shifts=shifts)
+    if feed == DIRECT:
+        for m, n in ((2, 2), (2, 130), (4, 2)):
+            check_outer(node, type_, out, [65, 0, 66, 129, 300], m, n, beta, pads=pads, shifts=shifts)
+
+
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+@pytest.mark.parametrize("slices", [1, 3, 16])
+def test_f64_outer(node, forced, beta, slices):
+    forced(64, slices)
+    check_outer(node, "f64", "f64", [300, 0, 1000, 65, 5, 777, 128, 1], 330, 140, beta, first=2, behind=3, pads=(1, 0, 3))
+    check_outer(node, "f64", "f64", [1] * 40 + [17, 0, 16, 33] * 8, 10, 7, beta, first=1, behind=1)
+
+
+@pytest.mark.parametrize("trans", ["T", "N"])
+@pytest.mark.parametrize("k", [1, 15, 333])
+def test_f64_product(node, forced, trans, k):
+    """The tile of 64 also where few outputs would take the other kernel."""
+    forced(64)
+    check_product(node, trans, "f64", [3, 0, 17, 1], 34, k, first=2, behind=3, pads=(1, 0, 3))
+
+
+@pytest.mark.parametrize("slices", [1, 5])
+def test_f64_outer_of_columns_far_apart(node, forced, slices):
+    """Columns more than 4 MB apart are read by another kernel, here over several slices with empty ones among them."""
+    import torch
+    forced(64, slices)
+    gen, sizes, m, n, ld = generator(91), [300, 0, 500, 20], 130, 70, (1 << 19) + 3
+    k = sum(sizes)
+    X = torch.empty(k, ld, dtype=torch.float64, device="cuda")[:, :m]
+    X.copy_(torch.randn(k, m, generator=gen, device="cuda", dtype=torch.float64))
+    Y = torch.randn(k, n, generator=gen, device="cuda", dtype=torch.float64)
+    for beta in (0.0, 0.5):
+        D = torch.ones(len(sizes), n, m, dtype=torch.float64, device="cuda")
+        assert node.grouped_outer_device(offsets_of(sizes), X, Y, D, beta=beta) == 0
+        for g, (x, y) in enumerate(zip(X.split(sizes), Y.split(sizes))):
+            ref, mag = y.T.contiguous() @ x + beta, y.T.abs().contiguous() @ x.abs() + beta
+            assert bool(((D[g] - ref).abs() <= (4 * sizes[g] + 8) * U * mag).all()), g
