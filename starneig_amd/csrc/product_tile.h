@@ -151,10 +151,10 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
     }
     // The bytes of the buffer: up to the last word of the operand (words, four bytes: the hardware tests each), where a chunk may reach it.  In the
     // last k-tile that is a chunk that starts in front of the end; MN, where a chunk is wider than the leading dimension, also one of the rows in front
-    // of them, which covers the next rows' numbers: up to EL rows.  Behind the last k-tile the buffer is empty.
+    // of them, which covers the next rows' numbers: up to EL rows.  Behind the last k-tile, and without outer positions, the buffer is empty.
     static __host__ __device__ __forceinline__ int bytes(int left, int outers, int ld)
     {
-        if (left <= 0) return 0;
+        if (left <= 0 || outers <= 0) return 0;
         if (left > (K ? O::KT : O::KT + O::EL)) return 0x7fffffff;
         int const rows = outers < ROWS ? outers : ROWS, wide = outers < ROWS + O::EL ? outers : ROWS + O::EL;
         return (K ? (rows - 1) * ld + left : (left - 1) * ld + wide) * (int)sizeof(T) + 3 & ~3;

@@ -44,7 +44,15 @@ template <> struct Mfma<signed char> {
 };
 
 // The columns [begin, end) of a group, or of the piece of a group that a workgroup takes.
-struct Span { int group, begin, end; };
+struct Span
+{
+    int group, begin, end;
+    __device__ __forceinline__ bool empty() const { return begin >= end; }
+};
+
+#ifdef SN_TEST_HOOKS
+__device__ int test_later_offsets;      // where the offsets are that more than 64 groups are walked over again, behind those that were counted
+#endif
 
 // Offsets come from the device (a router's prefix sums) and are not trusted: each is clamped to [0, n] and to its
 // predecessors' maximum, so that the groups are disjoint and inside the matrix whatever the array holds.
@@ -81,6 +89,9 @@ struct Pieces {
         start();
         for (int g0 = 0; g0 < groups; g0 += 64) walk(g0);
         total = before;
+#ifdef SN_TEST_HOOKS
+        if (groups > 64) offsets += test_later_offsets;
+#endif
     }
     __device__ __forceinline__ int offset(int g) const { return offsets ? min(max(offsets[g], 0), n) : g ? n : 0; }     // (none: one group of all columns)
     __device__ __forceinline__ void start() { carry = __builtin_amdgcn_readfirstlane(offset(0)); before = 0; }
@@ -96,7 +107,8 @@ struct Pieces {
         before += __builtin_amdgcn_readlane(sum, 63);
         carry = __builtin_amdgcn_readlane(end, 63);
     }
-    // Piece number `piece` < total.  (None of its columns where the offsets have changed meanwhile, which they must not.)
+    // Piece number `piece` < total.  Empty where the offsets of more than 64 groups have changed meanwhile, which they must not; the callers
+    // take it for no work, so that nothing is read or written outside the matrices.
     __device__ __forceinline__ Span at(int piece)
     {
         if (groups > 64) start();

@@ -68,7 +68,7 @@ void grouped_gemm_kernel(int groups, int m, int n, int k, int const *__restrict_
         row_and_column(t, rows, pieces.total, row, piece);
         Span const s = pieces.at(piece);
         int const r0 = row * P::BM;
-        p = Plan<T>{A + s.group * strideA + r0 * (P::A_K ? lda : 1L), B + s.begin * ldb, lda, ldb, m - r0, s.end - s.begin, k, r0, 0};
+        p = Plan<T>{A + s.group * strideA + r0 * (P::A_K ? lda : 1L), B + s.begin * ldb, lda, ldb, m - r0, s.end - s.begin, s.empty() ? 0 : k, r0, 0};
         return Place{s, true};
     }, [&](Plan<T> const &p, Place const &at) {
         tile.template store<T>(lds, [&](int x, int t, int y, int u, int r) { return (T)tile.acc[x][t][y][u][r]; },
@@ -186,7 +186,7 @@ void gemm_i8_kernel(int groups, int m, int n, int k, int const *__restrict__ off
         row_and_column(t, rows, pieces.total, row, piece);
         Span const s = pieces.at(piece);
         int const r0 = row * P::BM;
-        p = Plan<T>{A + s.group * strideA + r0 * lda, B + s.begin * ldb, lda, ldb, m - r0, s.end - s.begin, k, r0, 0};
+        p = Plan<T>{A + s.group * strideA + r0 * lda, B + s.begin * ldb, lda, ldb, m - r0, s.end - s.begin, s.empty() ? 0 : k, r0, 0};
         return Place{s, true};
     }, [&](Plan<T> const &p, Place const &at) {
         tile.template store<int>(lds, [&](int x, int t, int y, int u, int r) { return tile.acc[x][t][y][u][r]; },
@@ -312,6 +312,7 @@ void grouped_gemm_few_kernel(int groups, int m, int n, int k, int const *__restr
     int const t = tile_of_workgroup((m + 15) / 16 * pieces.total, 0);
     if (t < 0) return;
     Span const s = pieces.at((unsigned)t % (unsigned)pieces.total);
+    if (s.empty()) return;
     int const row = (unsigned)t / (unsigned)pieces.total;
     int const r0 = row * 16;
     few_columns_tile<T>(A + s.group * strideA + r0 * lda, lda, m - r0, B + s.begin * ldb, ldb, s.end - s.begin, k,
@@ -331,6 +332,7 @@ void grouped_dgemm_kernel(int groups, int m, int n, int k, int const *__restrict
     if (t < 0) return;
     int const row = (unsigned)t % (unsigned)rows;
     Span const s = pieces.at((unsigned)t / (unsigned)rows);
+    if (s.empty()) return;
     if constexpr (FAST) {
         __shared__ __attribute__((aligned(16))) char lds[DoubleTile<TA, true>::LDS_BYTES];
         long const r0 = row * 64;
@@ -357,6 +359,7 @@ void grouped_dgemm_few_kernel(int groups, int m, int n, int k, int const *__rest
     int const t = tile_of_workgroup((m + 15) / 16 * pieces.total, 0);
     if (t < 0) return;
     Span const p = pieces.at((unsigned)t % (unsigned)pieces.total);
+    if (p.empty()) return;
     int const r0 = (unsigned)t / (unsigned)pieces.total * 16, rows = m - r0, cols = p.end - p.begin;
     int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
     int const steps = (k + 7) / 8, run = (steps + WAVES - 1) / WAVES, first = min(wave * run, steps), end = min(first + run, steps);
@@ -646,6 +649,7 @@ void gemm_i8_few_kernel(int groups, int m, int n, int k, int const *__restrict__
     int const t = tile_of_workgroup((m + 15) / 16 * pieces.total, 0);
     if (t < 0) return;
     Span const s = pieces.at((unsigned)t % (unsigned)pieces.total);
+    if (s.empty()) return;
     int const row = (unsigned)t / (unsigned)pieces.total;
     int const r0 = row * 16;
     float const *const sa = scaleA + s.group * strideS + r0;
@@ -872,6 +876,9 @@ long sn_internal_product_reads_past(int size, int tile, int inner_contiguous, in
     return size == 1 ? reads_past<signed char>(tile, true, outers, k, ld) : size == 2 ? reads_past<__bf16>(tile, inner_contiguous, outers, k, ld)
         : inner_contiguous ? reads_past<double, 64, true>(outers, k, ld) : reads_past<double, 64, false>(outers, k, ld);
 }
+// From here on the offsets of more than 64 groups are looked up `ints` behind those that the pieces are counted from (as if they had changed meanwhile).
+extern "C" __attribute__((visibility("default")))
+int sn_internal_product_later_offsets(int ints) { return (int)hipMemcpyToSymbol(HIP_SYMBOL(sn::test_later_offsets), &ints, sizeof ints); }
 // From here on products by tiles of this size (64, 128, 256 where columns are aligned), sums over columns in this many slices (at least 1);
 // 0: as the rules have it.
 extern "C" __attribute__((visibility("default")))

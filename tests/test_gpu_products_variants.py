@@ -127,3 +127,55 @@ def test_f64_outer_of_columns_far_apart(node, forced, slices):
         for g, (x, y) in enumerate(zip(X.split(sizes), Y.split(sizes))):
             ref, mag = y.T.contiguous() @ x + beta, y.T.abs().contiguous() @ x.abs() + beta
             assert bool(((D[g] - ref).abs() <= (4 * sizes[g] + 8) * U * mag).all()), g
+
+
+LATER = {
+    "none": lambda sizes: [0] * (len(sizes) + 1),                       # every group empty
+    "behind": lambda sizes: [sum(sizes)] * (len(sizes) + 1),
+    "one": lambda sizes: [0] * len(sizes) + [sum(sizes) - 1],           # one group, a column less
+    "reversed": lambda sizes: [0, *(sum(sizes[:-g - 2:-1]) for g in range(len(sizes)))],
+}
+
+
+@pytest.mark.parametrize("later", list(LATER))
+@pytest.mark.parametrize("type_,tile,k,shift", [
+    ("bf16", 0, 200, 0), ("bf16", 0, 5, 1), ("bf16", 64, 200, 0), ("f16", 128, 200, 0), ("bf16", 256, 200, 0), ("bf16", 64, 200, 1), ("bf16", 128, 200, 1),
+    ("i8", 0, 200, 0), ("i8", 0, 5, 1), ("i8", 64, 200, 0), ("i8", 128, 200, 0), ("i8", 256, 200, 0), ("i8", 64, 201, 1), ("i8", 128, 201, 1),
+    ("f64", 0, 200, 0), ("f64", 64, 200, 0), ("f64", 64, 200, -1)])
+def test_offsets_that_change_during_a_call(node, forced, library, type_, tile, k, shift, later):
+    """More than 64 groups, whose offsets are walked over again for every tile, and are others then: nothing is promised about the columns of C, but
+    nothing else is written, and where no group has a column any more, nothing at all.  (shift -1: columns more than 4 MB apart.)"""
+    import torch
+    forced(tile)
+    sizes = [1] * 50 + [0, 3, 0, 0, 9] * 12 + [40]
+    groups, n, m, pad = len(sizes), sum(sizes), 150, 4
+    counted = offsets_of(sizes)
+    both = torch.cat([counted, torch.tensor(LATER[later](sizes), dtype=torch.int32, device="cuda")])
+    dtype = {"i8": torch.int8}.get(type_) or kind(type_)
+    one = lambda rows: torch.ones(rows * k + 1, dtype=dtype, device="cuda")[max(shift, 0):][:rows * k].view(rows, k)
+    A, B = one(m)[None].expand(groups, m, k), one(n)
+    if shift < 0:
+        far = torch.empty(n, (1 << 19) + 3, dtype=dtype, device="cuda")
+        B = far[:, :k].fill_(1)
+    C = torch.full((n + 2 * pad, m + pad), 7.0, dtype=torch.float32 if type_ == "i8" else dtype, device="cuda")
+    inner = C[pad:-pad, :m]
+    scale = torch.ones(max(n, m), device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    assert library.sn_internal_product_later_offsets(groups + 1) == 0
+    try:
+        if type_ == "i8":
+            assert library.starneig_amd_grouped_gemm_i8_device(
+                node.AMD_F32, groups, m, n, k, both.data_ptr(), A.data_ptr(), k, 0, scale.data_ptr(), 0, B.data_ptr(), k, scale.data_ptr(),
+                inner.data_ptr(), m + pad, stream) == 0
+        else:
+            assert node.grouped_gemm_device("T", both[:groups + 1], A, B, inner) == 0
+        torch.cuda.synchronize()
+    finally:
+        assert library.sn_internal_product_later_offsets(0) == 0
+    if later in ("none", "behind"):
+        assert bool((inner == 7.0).all())
+    else:
+        assert bool(((inner == 7.0) | (inner == float(k))).all())
+    inner.fill_(7.0)
+    assert bool((C == 7.0).all())

@@ -40,3 +40,12 @@ def test_no_load_reads_past_the_operand_f64(outers):
             assert past(8, 64, 0, outers, k, ld) == 0, (ld, k)
         for ld in (k, k + 1, k + 5):
             assert past(8, 64, 1, outers, k, ld) == 0, (ld, k)
+
+
+@pytest.mark.parametrize("size,tile", [(1, 64), (1, 256), (2, 64), (2, 128), (2, 256), (8, 64)])
+@pytest.mark.parametrize("inner_contiguous", [0, 1])
+def test_no_load_reads_an_operand_without_columns(size, tile, inner_contiguous):
+    """A tile of no columns, as offsets leave it that change during a call."""
+    for k in (1, 3, 64, 65, 200):
+        for ld in (4, 200, 204, 4096):
+            assert past(size, tile, inner_contiguous, 0, k, ld) == 0, (k, ld)
