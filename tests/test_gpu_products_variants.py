@@ -1,6 +1,7 @@
 """GPU: every variant of the products' tiles, whatever the rules that choose among them: tile, feed and slices are forced through the
 test-support library, with several tiles a workgroup, inner lengths that cut a chunk in the first, a middle and the last k-tile, and
-sums that are added to what is there.  Bounds as in test_gpu_products.py."""
+sums that are added to what is there; and the rounding to 8 bits at the lengths where its kernels change.  Bounds as in test_gpu_products.py."""
+import numpy as np
 import pytest
 
 from helpers import U
@@ -80,7 +81,7 @@ def test_8_bit_product(node, forced, out, tile, pad, shift, k):
         assert bool((C[:, m:] == 7.0).all()) and bool((C[:first] == 7.0).all()) and bool((C[n - behind:] == 7.0).all())
 
 
-@pytest.mark.parametrize("type_,out", [("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("type_,out", [("bf16", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "f32")])
 @pytest.mark.parametrize("beta", [0.0, 0.5])
 @pytest.mark.parametrize("slices", [1, 2, 7, 64])
 @pytest.mark.parametrize("tile,feed", [(64, DIRECT), (128, DIRECT), (256, DIRECT), (64, STAGED), (128, STAGED)])
@@ -127,6 +128,20 @@ def test_f64_outer_of_columns_far_apart(node, forced, slices):
         for g, (x, y) in enumerate(zip(X.split(sizes), Y.split(sizes))):
             ref, mag = y.T.contiguous() @ x + beta, y.T.abs().contiguous() @ x.abs() + beta
             assert bool(((D[g] - ref).abs() <= (4 * sizes[g] + 8) * U * mag).all()), g
+
+
+@pytest.mark.parametrize("type_", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("k", [1024, 1025, 2048, 2049, 4096, 4097, 5001, 8192, 8193, 32768, 32769])
+def test_quantize_i8_on_both_sides_of_each_kernel(node, type_, k):
+    import torch
+    n = 9
+    X = torch.randn(n, k, generator=generator(k), device="cuda", dtype=torch.float64).mul_(3).to(kind(type_))
+    Q, scale = torch.empty(n, k, dtype=torch.int8, device="cuda"), torch.empty(n, device="cuda")
+    assert node.quantize_i8_device(X, Q, scale) == 0
+    x = X.float().cpu().numpy()
+    s = np.abs(x).max(axis=1) / np.float32(127)
+    assert np.array_equal(scale.cpu().numpy(), s)
+    assert np.array_equal(Q.cpu().numpy(), np.rint(x / s[:, None]).astype(np.int8))
 
 
 LATER = {
