@@ -546,14 +546,14 @@ static double outer_time(Cut c, bool fast, long groups, long m, long n, long k)
     long const items = groups * ((m + c.tile - 1) / c.tile) * ((n + c.tile - 1) / c.tile) * c.slices;
     return tile_time(c.tile, fast, items, (double)k / groups / c.slices / 64) + (c.slices > 1 ? 3 + c.slices * (double)groups * m * n * 8 / 4e6 : 0);
 }
-static Cut outer_cut(bool fast, long groups, long m, long n, long k)
+static Cut outer_cut(bool fast, long groups, long m, long n, long k, int most_slices = 64)
 {
     Cut best = {128, 1};
-    if (forced_tile) return Cut{forced_tile, forced_slices};
+    if (forced_tile) return Cut{forced_tile, std::min(forced_slices, most_slices)};
     for (int tile : {256, 128, 64})
         for (int slices : {1, 2, 4, 8, 16, 32, 64}) {
             Cut const c = {tile, slices};
-            if ((tile == 256 && !fast) || (slices > 1 && k / groups / slices < 64)) continue;
+            if (slices > most_slices || (tile == 256 && !fast) || (slices > 1 && k / groups / slices < 64)) continue;
             if (outer_time(c, fast, groups, m, n, k) < outer_time(best, fast, groups, m, n, k)) best = c;
         }
     return best;
@@ -587,7 +587,9 @@ static hipError_t outer_launch(hipStream_t s, int groups, int m, int n, int k, i
             m, n, k, offsets, (T const *)X, (long)ldx, (T const *)Y, (long)ldy, (float)beta, (D *)out, (long)ldd, strideD);
     Cut c = outer_cut(fast, groups, m, n, k);
     long const plane = (long)groups * m * n * 4;
-    if (c.slices > 1 && (work == nullptr || work_size < c.slices * plane)) c.slices = 1;
+    // (the tile that is best with slices need not be without: 36501 columns, 1050 x 666: 256 with 16 slices, 64 with
+    // one, which takes 168 us instead of 665)
+    if (c.slices > 1 && (work == nullptr || work_size < c.slices * plane)) c = outer_cut(fast, groups, m, n, k, 1);
     auto const go = [&](auto *to, int ld, long stride, double b) {
         typedef std::remove_pointer_t<decltype(to)> O;
         auto const launch = c.tile == 256 ? outer_tiles<T, O, ProductTile<T, 256, 256, 2, 4, false, false, DIRECT>>
@@ -879,6 +881,17 @@ long sn_internal_product_reads_past(int size, int tile, int inner_contiguous, in
 // From here on the offsets of more than 64 groups are looked up `ints` behind those that the pieces are counted from (as if they had changed meanwhile).
 extern "C" __attribute__((visibility("default")))
 int sn_internal_product_later_offsets(int ints) { return (int)hipMemcpyToSymbol(HIP_SYMBOL(sn::test_later_offsets), &ints, sizeof ints); }
+// The tile and the slices of a gradient with aligned or other columns, with scratch memory for so many slices or none (most_slices 1): slices * 1000 + tile
+extern "C" __attribute__((visibility("default")))
+int sn_internal_product_outer_cut(int aligned, int groups, int m, int n, int k, int most_slices)
+{
+    sn::Cut const c = sn::outer_cut(aligned, groups, m, n, k, most_slices);
+    return c.slices * 1000 + c.tile;
+}
+// What the rules take a gradient's launch for, in us
+extern "C" __attribute__((visibility("default")))
+double sn_internal_product_outer_time(int tile, int slices, int aligned, int groups, int m, int n, int k)
+{ return sn::outer_time(sn::Cut{tile, slices}, aligned, groups, m, n, k); }
 // From here on products by tiles of this size (64, 128, 256 where columns are aligned), sums over columns in this many slices (at least 1);
 // 0: as the rules have it.
 extern "C" __attribute__((visibility("default")))

@@ -96,6 +96,28 @@ def test_outer(node, forced, type_, out, beta, slices, tile, feed):
             check_outer(node, type_, out, [65, 0, 66, 129, 300], m, n, beta, pads=pads, shifts=shifts)
 
 
+def test_outer_without_scratch_memory_has_the_tile_that_is_best_without(node, forced, library):
+    """With scratch memory the rules take tiles of 256 here, without it those of 64, whose four parts of the sum show in the last bits."""
+    import torch
+    k, m, n = 36501, 1050, 666
+    assert library.sn_internal_product_outer_cut(1, 1, m, n, k, 64) % 1000 != 64 and library.sn_internal_product_outer_cut(1, 1, m, n, k, 1) == 1064
+    gen = generator(7)
+    X, Y = (torch.randn(k, s, generator=gen, device="cuda").bfloat16() for s in (m, n))
+    off, stream = offsets_of([k]), torch.cuda.current_stream().cuda_stream
+
+    def result():
+        D = torch.empty(n, m, device="cuda")
+        assert library.starneig_amd_grouped_outer_device(node.AMD_BF16, node.AMD_F32, 1, m, n, k, off.data_ptr(), X.data_ptr(), m, Y.data_ptr(), n, 0.0,
+                                                         D.data_ptr(), m, m * n, None, 0, stream) == 0
+        return D
+
+    by_rule, by_tile = result(), {}
+    for tile in (64, 128):
+        forced(tile)
+        by_tile[tile] = result()
+    assert torch.equal(by_rule, by_tile[64]) and not torch.equal(by_rule, by_tile[128])
+
+
 @pytest.mark.parametrize("beta", [0.0, 0.5])
 @pytest.mark.parametrize("slices", [1, 3, 16])
 def test_f64_outer(node, forced, beta, slices):
