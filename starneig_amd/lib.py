@@ -545,8 +545,9 @@ def _product_device(t):
     return device, torch[5](device)
 
 
-def _product_matrix(name, t, shape, dtype, device):
-    """(pointer, leading dimension, stride of the groups) of a tensor of this shape and type on this device."""
+def _product_matrix(name, t, shape, dtype, device, vectors=False):
+    """(pointer, leading dimension, stride of the groups) of a tensor of this shape and type on this device.  vectors: its rows
+    are one vector a group, at any distance (0 where a tensor is expanded over the groups)."""
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
     if t.dtype != dtype:
@@ -559,6 +560,8 @@ def _product_matrix(name, t, shape, dtype, device):
         raise ValueError(f"the last dimension of {name} is not contiguous")
     if dims == 1:
         return t.data_ptr(), rows, 0
+    if vectors:
+        return t.data_ptr(), rows, (stride[0] if shape[0] > 1 else 0)
     # (the stride of a dimension of one entry says nothing)
     ld = stride[-2] if shape[-2] > 1 else rows or 1
     if ld < rows or ld > 0x7fffffff:
@@ -642,7 +645,7 @@ def gemm_i8_device(tA, tScaleA, tB, tScaleB, tC):
 
 
 def grouped_gemm_i8_device(tOffsets, tA, tScaleA, tB, tScaleB, tC):
-    """The same with tA (groups, m, k) and tScaleA (groups, m) for the columns of every group."""
+    """The same with tA (groups, m, k) and tScaleA (groups, m) for the columns of every group; either may be expanded over the groups."""
     device, stream = _product_device(tB)
     _, _, i8, f32, _, _ = _product_torch
     poff, groups = _product_offsets(tOffsets, device)
@@ -651,10 +654,10 @@ def grouped_gemm_i8_device(tOffsets, tA, tScaleA, tB, tScaleB, tC):
     pb, ldb, _ = _product_matrix("B", tB, shape, i8, device)
     pc, ldc, _ = _product_matrix("C", tC, (n, m), tC.dtype, device)
     pa, lda, stride = _product_matrix("A", tA, (groups, m, k), i8, device)
-    psa, ldsa, _ = _product_matrix("scaleA", tScaleA, (groups, m), f32, device)
+    psa, _, strides = _product_matrix("scaleA", tScaleA, (groups, m), f32, device, vectors=True)
     psb, _, _ = _product_matrix("scaleB", tScaleB, (n,), f32, device)
     return load().starneig_amd_grouped_gemm_i8_device(
-        _product_type(tC), groups, m, n, k, poff, pa, lda, stride, psa, ldsa if groups > 1 else 0, pb, ldb, psb, pc, ldc, stream)
+        _product_type(tC), groups, m, n, k, poff, pa, lda, stride, psa, strides, pb, ldb, psb, pc, ldc, stream)
 
 
 def lcg_fill_device(t, m, n, seed=2019, mode=0):
