@@ -33,12 +33,16 @@ __device__ __forceinline__ i32x4 buffer(void const *p, int bytes)
 // 16 bytes a lane from `offset` of the buffer into LDS: the wave's from `to` (the same in all lanes) on, in the lanes' order.  In assembly: with the
 // builtin the compiler waits for all loads before the next transposing LDS read, which it takes to read what they write; here the
 // barriers order them.  The compiler does not look inside, so the five wait states are here that a load needs behind a vector
-// instruction (v_readfirstlane) that has written one of its scalar registers, and the one behind m0.
+// instruction (v_readfirstlane) that has written one of its scalar registers, and the one behind m0.  m0 is named as written, so that no
+// value of the compiler's own is taken to outlast the statement (it warns that it never allocates m0, which holds).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(i32x4 buffer, unsigned offset, int to)
 {
     i32x4 const b = {uniform(buffer.x), uniform(buffer.y), uniform(buffer.z), uniform(buffer.w)};
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(uniform(to)), "v"(offset), "s"(b) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(uniform(to)), "v"(offset), "s"(b) : "m0", "memory");
 }
+#pragma clang diagnostic pop
 // threadIdx.x for what is computed once a tile: the compiler must not compute it before the loops and hold it in registers meanwhile
 __device__ __forceinline__ int thread_now() { int t = threadIdx.x; asm volatile("" : "+v"(t)); return t; }
 // number of the wave, of the threads that share a tile
