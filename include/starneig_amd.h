@@ -181,6 +181,8 @@ starneig_error_t starneig_amd_grouped_outer_device(
 long starneig_amd_grouped_outer_work_size(int type, int groups, int m, int n, int k);
 
 /* Q(:, c) = rint(X(:, c) / s_c), s_c = dScale[c] = max_i |X(i, c)| / 127 in IEEE fp32, halves to even.  X: k x n of type F32, BF16 or F16.
+ * Q is limited to [-127, 127]: where s_c is an fp32 subnormal its own rounding is coarse, and the quotient of an F32 column can be larger (up to 190: a
+ * maximum of 190 smallest subnormals has s_c = 1 of them).
  * A column of zeros (or whose s underflows to 0) gets s = 0 and Q = 0; one that holds an infinity or a NaN gets that s and Q = 0 (its product is NaN). */
 starneig_error_t starneig_amd_quantize_i8_device(
     int type, int k, int n, void const *dX, int ldX, signed char *dQ, int ldQ, float *dScale, void *stream);

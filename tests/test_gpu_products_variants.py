@@ -166,6 +166,33 @@ def test_quantize_i8_on_both_sides_of_each_kernel(node, type_, k):
     assert np.array_equal(Q.cpu().numpy(), np.rint(x / s[:, None]).astype(np.int8))
 
 
+@pytest.mark.parametrize("type_", ["bf16", "f32"])
+@pytest.mark.parametrize("k", [300, 5001, 33000])
+def test_quantize_i8_of_tiny_and_huge_columns(node, type_, k):
+    """Maxima from the smallest subnormal, where the quotient passes 127 and is limited, over the ends of the range in which the quotient comes from the
+    reciprocal (scales of 2^-100 and 2^100), to the largest number."""
+    import torch
+    dtype = kind(type_)
+    step = float(torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps)           # the smallest subnormal
+    tops = [step * j for j in (1, 63, 64, 127, 190, 191, 254, 255, 317, 318, 1000, 12345)]
+    tops += [127 * 2.0 ** e * f for e in (-127, -126, -125, -101, -100, -99, 99, 100, 101, 120) for f in (1 - 2 ** -7, 1.0, 1 + 2 ** -7)]
+    tops += [torch.finfo(dtype).max]
+    gen = generator(k)
+    X = torch.rand(len(tops), k, generator=gen, device="cuda", dtype=torch.float64).mul_(2).sub_(1)
+    X[:, k // 2] = 1.0
+    X = (X * torch.tensor(tops, dtype=torch.float64, device="cuda")[:, None]).to(dtype)
+    Q, scale = torch.full((len(tops), k), 99, dtype=torch.int8, device="cuda"), torch.empty(len(tops), device="cuda")
+    assert node.quantize_i8_device(X, Q, scale) == 0
+    x = X.float().cpu().numpy()
+    s = np.abs(x).max(axis=1) / np.float32(127)
+    assert np.array_equal(scale.cpu().numpy(), s)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        q = np.where(s[:, None] > 0, np.clip(np.rint(x / s[:, None]), -127, 127), 0)
+    assert np.array_equal(Q.cpu().numpy(), q.astype(np.int8))
+    # some of them are limited, in fp32 only: the smallest bf16 has a scale of 516 smallest fp32 subnormals, which half of one moves by less than a thousandth
+    assert (np.abs(x).max(axis=1)[s > 0] / s[s > 0] > 127.5).any() == (type_ == "f32")
+
+
 LATER = {
     "none": lambda sizes: [0] * (len(sizes) + 1),                       # every group empty
     "behind": lambda sizes: [sum(sizes)] * (len(sizes) + 1),
