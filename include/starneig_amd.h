@@ -142,13 +142,13 @@ starneig_error_t starneig_amd_dgemm_device(
     double *dC, int ldC, void *stream);
 
 /* ---- products over ragged groups of columns, and in 8-bit integers ---------------------------------------
- * The products of layers that have a matrix per group of columns (experts and the tokens sent to them, windows and
- * the columns right of them).  Column-major like everything here: a token is a column, so a row-major array
- * (tokens, features) is passed as it lies, and row-major weights (out, in) are A with transA = 'T'.
+ * The products of layers that have a matrix per group of columns (experts and the tokens sent to them).  Column-major like everything here: a token is a
+ * column, so a row-major array (tokens, features) is passed as it lies, and row-major weights (out, in) are A with transA = 'T'.
  * Group g owns the columns [dOffsets[g], dOffsets[g + 1]) of the n columns; dOffsets holds groups + 1 ints in DEVICE
  * memory and may be written on `stream` just before (prefix sums of a router's counts): the host does not read it.
  * Groups may be empty; columns in front of the first and behind the last group belong to none.  An offset outside
- * [0, n] counts as the nearer end, one below its predecessor as its predecessor.
+ * [0, n] counts as the nearer end, one below its predecessor as its predecessor.  They must not change until the call has finished on the device:
+ * where they do, nothing is read or written outside the matrices, but nothing more is promised.
  * The calls enqueue on `stream` and return; they hold no state and no lock, so they may run
  * on several streams at once and be captured into graphs.  All pointers are on the current device and aligned to their
  * elements; outputs must not overlap inputs; m, n and k are at most 2^30, groups
@@ -169,7 +169,8 @@ starneig_error_t starneig_amd_grouped_gemm_device(
 
 /* D_g = X_g Y_g^T + beta D_g, the sum over the columns of group g: the gradient of A_g with X = B and Y = the gradient
  * of C (transA = 'T'), or X and Y swapped ('N').  X: m x k, Y: n x k (k: all columns), D_g: m x n at dD + g strideD
- * elements.  An empty group gives beta D_g; beta = 0 does not read D.  typeD: `type`, or F32 for BF16 / F16.
+ * elements, strideD at least (n - 1) ldD + m for more than one group.  An empty group gives beta D_g; beta = 0 does not read D.  typeD: `type`, or F32 for
+ * BF16 / F16.  beta is taken in fp32 for these two types.
  * dWork: scratch memory of the call's own (two captured graphs that may run at once need two), 16-byte aligned, of workSize bytes.  With
  * starneig_amd_grouped_outer_work_size bytes of it a long sum over few outputs is cut into parts that run at once; with less, or NULL, it is
  * not cut: slower, and rounded differently. */
