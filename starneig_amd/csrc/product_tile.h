@@ -156,10 +156,11 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
     // The bytes of the buffer: up to the last word of the operand (words, four bytes: the hardware tests each), where a chunk may reach it.  In the
     // last k-tile that is a chunk that starts in front of the end; MN, where a chunk is wider than the leading dimension, also one of the rows in front
     // of them, which covers the next rows' numbers: up to EL rows.  Behind the last k-tile, and without outer positions, the buffer is empty.
+    static constexpr int REACH = K ? O::KT : O::KT + O::EL, WHOLE = 0x7fffffff;
     static __host__ __device__ __forceinline__ int bytes(int left, int outers, int ld)
     {
+        if (left > REACH) return WHOLE;
         if (left <= 0 || outers <= 0) return 0;
-        if (left > (K ? O::KT : O::KT + O::EL)) return 0x7fffffff;
         int const rows = outers < ROWS ? outers : ROWS, wide = outers < ROWS + O::EL ? outers : ROWS + O::EL;
         return (K ? (rows - 1) * ld + left : (left - 1) * ld + wide) * (int)sizeof(T) + 3 & ~3;
     }
@@ -176,13 +177,17 @@ struct Stream<T, ROWS, K, THREADS, DIRECT> {
     __device__ __forceinline__ void begin(int kt)
     {
         int const left = k - kt * O::KT;
-        if (left <= O::KT && left > 0) {
-            int const thread = thread_now() % THREADS;
-            #pragma unroll
-            for (int s = 0; s < O::LOADS; s++)
-                if (behind(s * THREADS + thread, left)) at[s] = NOTHING;
+        int size = WHOLE;
+        if (left <= REACH) {            // (one branch in all other k-tiles)
+            size = bytes(left, outers, ld);
+            if (left <= O::KT) {
+                int const thread = thread_now() % THREADS;
+                #pragma unroll
+                for (int s = 0; s < O::LOADS; s++)
+                    if (behind(s * THREADS + thread, left)) at[s] = NOTHING;
+            }
         }
-        from = buffer(K ? base + (long)kt * O::KT : base + kt * step, bytes(left, outers, ld));
+        from = buffer(K ? base + (long)kt * O::KT : base + kt * step, size);
     }
     __device__ __forceinline__ void load(int lds, int s) const { load_to_lds(from, at[s], lds + wave_number() % (THREADS / 64) * 1024 + s * THREADS * 16); }
     __device__ __forceinline__ void fetch(int lds, int kt)

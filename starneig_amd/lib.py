@@ -545,9 +545,8 @@ def _product_device(t):
     return device, torch[5](device)
 
 
-def _product_matrix(name, t, shape, dtype, device, vectors=False):
-    """(pointer, leading dimension, stride of the groups) of a tensor of this shape and type on this device.  vectors: its rows
-    are one vector a group, at any distance (0 where a tensor is expanded over the groups)."""
+def _product_matrix(name, t, shape, dtype, device):
+    """(pointer, leading dimension, stride of the groups) of a tensor of this shape and type on this device."""
     if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
     if t.dtype != dtype:
@@ -560,13 +559,20 @@ def _product_matrix(name, t, shape, dtype, device, vectors=False):
         raise ValueError(f"the last dimension of {name} is not contiguous")
     if dims == 1:
         return t.data_ptr(), rows, 0
-    if vectors:
-        return t.data_ptr(), rows, (stride[0] if shape[0] > 1 else 0)
     # (the stride of a dimension of one entry says nothing)
     ld = stride[-2] if shape[-2] > 1 else rows or 1
     if ld < rows or ld > 0x7fffffff:
         raise ValueError(f"the columns of {name} overlap or lie 2^31 entries apart")
     return t.data_ptr(), ld, (stride[0] if dims == 3 and shape[0] > 1 else 0)
+
+
+def _product_vectors(name, t, shape, dtype, device):
+    """(pointer, stride of the groups) of one vector a group, which may lie at any distance (0: expanded over the groups)."""
+    groups, entries = shape
+    if groups > 1 and t.shape == shape and t.stride(0) < entries:
+        return _product_matrix(name, t[0], (entries,), dtype, device)[0], t.stride(0)
+    pointer, stride, _ = _product_matrix(name, t, shape, dtype, device)
+    return pointer, stride if groups > 1 else 0
 
 
 def _product_sizes(name, t):
@@ -654,7 +660,7 @@ def grouped_gemm_i8_device(tOffsets, tA, tScaleA, tB, tScaleB, tC):
     pb, ldb, _ = _product_matrix("B", tB, shape, i8, device)
     pc, ldc, _ = _product_matrix("C", tC, (n, m), tC.dtype, device)
     pa, lda, stride = _product_matrix("A", tA, (groups, m, k), i8, device)
-    psa, _, strides = _product_matrix("scaleA", tScaleA, (groups, m), f32, device, vectors=True)
+    psa, strides = _product_vectors("scaleA", tScaleA, (groups, m), f32, device)
     psb, _, _ = _product_matrix("scaleB", tScaleB, (n,), f32, device)
     return load().starneig_amd_grouped_gemm_i8_device(
         _product_type(tC), groups, m, n, k, poff, pa, lda, stride, psa, strides, pb, ldb, psb, pc, ldc, stream)
