@@ -449,7 +449,7 @@ static hipError_t dgemm_launch(hipStream_t s, int groups, int m, int n, int k, i
 {
     long const tiles = most_pieces(groups, n, 64) * ((m + 63) / 64);
     if (tiles >= 1L << 31) return hipErrorInvalidConfiguration;
-    // In us, fitted to 1 ... 640 columns, 426 ... 1152 rows and 300 ... 4096 inner terms.  1 column, 768 x 2624: 19 us (tiles of 64: 117 us); 64 columns, 512 x 512: 10 us
+    // In us, fitted to 1 ... 640 columns, 426 ... 1152 rows and 300 ... 4096 inner terms; elsewhere an extrapolation.  1 column, 768 x 2624: 19 us (tiles of 64: 117 us); 64 columns, 512 x 512: 10 us
     // (26 us); 576 columns, 512 x 4096: 143 us (180 us); 512 columns, 512 x 300: 21 us (17 us)
     long const small = most_pieces(groups, n, 16) * ((m + 15) / 16);
     if (k > 0 && !forced_tile && 10 + 3.4e-5 * small * k < 6 + 0.0425 * k * std::max(1.0, tiles / 256.0) && small < 1L << 22)
@@ -470,7 +470,8 @@ static unsigned resident(long tiles)
 
 // What a launch takes, in us, fitted to launches of 64 ... 65536 columns, 1 ... 32 groups, 64 ... 4096 rows and 256 ... 8192 inner terms: rounds of the
 // workgroups that the chip holds at once, each of so many k-tiles and what it takes to begin and to store a tile.  A k-tile takes as long as the
-// memory's latency while few workgroups run, as long as the matrix cores need when they fill the chip.
+// memory's latency while few workgroups run, as long as the matrix cores need when they fill the chip.  (Measured with 16-bit numbers; a k-tile of 8-bit ones has
+// as many bytes, takes as many instructions, and is taken for as long.)
 //   tile  64: four waves cut the inner index, for products of few outputs;   200 columns, 512 x 8192:  26 us (128: 74 us)
 //   tile 128: two workgroups a compute unit;                                2048 columns, 4096 x 4096: 73 us (64: 124 us, 256: 89 us)
 //   tile 256: the fewest reads a product;                                   4096 columns, 4096 x 4096: 120 us (128: 143 us)
@@ -498,7 +499,7 @@ static int product_tile(bool fast, int groups, int m, int n, int ktiles)
     return best;
 }
 // Few columns a group on average, and too few 64 x 64 tiles to fill the chip: 16 columns, 4096 x 4096: 11 us, in tiles of 64 15 us; 256 columns of 32
-// groups, 2048 x 1408: 62 us, in tiles of 128 32 us.
+// groups, 2048 x 1408: 62 us, in tiles of 128 36 us.
 static bool few_columns(int groups, int m, int n) { return !forced_tile && (long)n <= 16L * groups && most_pieces(groups, n, 64) * ((m + 63) / 64) < 256; }
 
 template <typename T, typename P>
@@ -702,7 +703,7 @@ hipError_t gemm_i8(hipStream_t s, ProductType typeC, int groups, int m, int n, i
 // by its remainder: the first leaves it within one unit, and from there the second rounds correctly (Markstein's theorem
 // on division by multiply-add); a third of the compiler's full division.  Adding 3 * 2^22 rounds to an integer, halves to even, whose low
 // byte is then q.
-// 8192 columns of 4096 bf16 numbers: 18 us, 5.5 TB/s of reads and writes.
+// 8192 columns of 4096 bf16 numbers: 18 - 19 us, 5.4 TB/s of reads and writes.
 template <typename T> struct Eight;         // eight numbers as they lie in memory
 template <> struct Eight<float> {
     u32x4 v[2];
