@@ -10,7 +10,7 @@ CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
 
 @pytest.mark.parametrize("path", sorted(glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.hip"))), ids=os.path.basename)
 def test_registers_that_inline_assembly_writes_are_clobbers(path):
-    for statement in re.findall(r"\basm\b.*?;\s*$", open(path).read(), re.M | re.S):
+    for statement in re.findall(r"\basm\b\s*(?:volatile\s*)?\(.*?\);", open(path).read(), re.S):
         strings = re.findall(r'"((?:[^"\\]|\\.)*)"', statement)
         for line in re.split(r"\\n(?:\\t)?", strings[0]):
             written = re.match(r"\s*[sv]_\w+\s+(m0|vcc|exec|scc|[sv]\d+)\b", line)
